@@ -1,12 +1,13 @@
-"""ctypes loader for libcap2det_hip.so (the C-ABI of include/cap2det_hip.h).
+"""ctypes loader for libcap2det_hip.so (the C-ABI of include/cap2det_hip.h and, for the grouped and 8-bit
+matrix products, include/cap2det_products.h).
 
 There is NO CPU fallback: if the shared library is missing or a symbol is absent the
 product path raises.  `import torch` happens first so that the HIP runtime the library binds
 to (soname libamdhip64.so.7) is the one PyTorch already loaded — device pointers and streams
 are then shared between torch and the kernels.
 
-Argument types are taken from the declarations in include/cap2det_hip.h itself, so the
-binding cannot drift from the header.
+Argument types are taken from the declarations in the headers themselves, so the binding cannot drift
+from them.
 """
 import ctypes
 import os
@@ -18,9 +19,11 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 # library.
 LIB_PATH = os.environ.get("C2D_LIB") or os.path.join(_HERE, "csrc", "libcap2det_hip.so")
 HEADER_PATH = os.path.join(os.path.dirname(_HERE), "include", "cap2det_hip.h")
+PRODUCTS_HEADER_PATH = os.path.join(os.path.dirname(_HERE), "include", "cap2det_products.h")
 
 _lib = None
 _SIGS = None
+_PRODUCT_SIGS = None
 
 
 class Cap2DetHipError(RuntimeError):
@@ -38,30 +41,47 @@ def _ctype(decl):
           "unsigned int": ctypes.c_uint, "void": None}[base]
 
 
-def header_signatures():
-  """Parses `int c2d_xxx(...)` declarations of the header -> {name: (restype, [argtypes])}."""
-  global _SIGS
-  if _SIGS is not None:
-    return _SIGS
-  with open(HEADER_PATH) as f:
+def _parse_header(path, prefix):
+  with open(path) as f:
     text = re.sub(r"/\*.*?\*/", "", f.read(), flags=re.S)
   sigs = {}
-  for m in re.finditer(r"(const char\*|unsigned long long|unsigned int|long long|int)\s+(c2d_\w+)"
-                       r"\s*\(([^)]*)\)\s*;", text):
+  for m in re.finditer(r"(const char\*|unsigned long long|unsigned int|long long|int)\s+(%s_\w+)"
+                       r"\s*\(([^)]*)\)\s*;" % prefix, text):
     ret, name, params = m.group(1), m.group(2), m.group(3).strip()
     args = [] if params in ("void", "") else [_ctype(p) for p in params.split(",")]
     restype = {"int": ctypes.c_int, "long long": ctypes.c_longlong,
                "unsigned int": ctypes.c_uint,
                "unsigned long long": ctypes.c_ulonglong}.get(ret, ctypes.c_char_p)
     sigs[name] = (restype, args)
-  _SIGS = sigs
   return sigs
+
+
+def header_signatures():
+  """Parses `int c2d_xxx(...)` declarations of the header -> {name: (restype, [argtypes])}."""
+  global _SIGS
+  if _SIGS is None:
+    _SIGS = _parse_header(HEADER_PATH, "c2d")
+  return _SIGS
+
+
+def product_signatures():
+  """The same of the `c2dp_xxx` declarations of include/cap2det_products.h."""
+  global _PRODUCT_SIGS
+  if _PRODUCT_SIGS is None:
+    _PRODUCT_SIGS = _parse_header(PRODUCTS_HEADER_PATH, "c2dp")
+  return _PRODUCT_SIGS
 
 
 def header_abi_version():
   """`#define C2D_ABI_VERSION n` of the header."""
   with open(HEADER_PATH) as f:
     return int(re.search(r"#define\s+C2D_ABI_VERSION\s+(\d+)", f.read()).group(1))
+
+
+def product_abi_version():
+  """`#define C2DP_ABI_VERSION n` of include/cap2det_products.h."""
+  with open(PRODUCTS_HEADER_PATH) as f:
+    return int(re.search(r"#define\s+C2DP_ABI_VERSION\s+(\d+)", f.read()).group(1))
 
 
 def load():
@@ -75,15 +95,15 @@ def load():
         "g.build()'` (or `make -C cap2det_amd/csrc`). There is no CPU fallback." % LIB_PATH)
   import torch  # noqa: F401  (loads the HIP runtime first, see module docstring)
   lib = ctypes.CDLL(LIB_PATH, mode=ctypes.RTLD_GLOBAL)
-  for name, (restype, argtypes) in header_signatures().items():
+  for name, (restype, argtypes) in list(header_signatures().items()) + list(product_signatures().items()):
     fn = getattr(lib, name)  # AttributeError => header/library mismatch: fail loudly
     fn.restype = restype
     fn.argtypes = argtypes
-  want = header_abi_version()
-  got = lib.c2d_version()
-  if got != want:
-    raise ImportError("cap2det_amd: %s was built for ABI %d, include/cap2det_hip.h declares %d — "
-                      "rebuild it (`make -C cap2det_amd/csrc`)" % (LIB_PATH, got, want))
+  for header, want, got in (("cap2det_hip.h", header_abi_version(), lib.c2d_version()),
+                            ("cap2det_products.h", product_abi_version(), lib.c2dp_version())):
+    if got != want:
+      raise ImportError("cap2det_amd: %s was built for ABI %d, include/%s declares %d — "
+                        "rebuild it (`make -C cap2det_amd/csrc`)" % (LIB_PATH, got, header, want))
   _lib = lib
   return lib
 

@@ -11,8 +11,9 @@
 // tensors: base pointer of the slot + the recorded offset) and scalar arguments bound to a slot
 // (dropout key, learning rate).
 //
-// Entry points are reached through typed thunks generated from the header (plan_thunks.inc).
+// Entry points are reached through typed thunks generated from the headers (plan_thunks.inc).
 #include "c2d_common.h"
+#include "../../include/cap2det_products.h"
 #include <string.h>
 #include <stdlib.h>
 #include <algorithm>

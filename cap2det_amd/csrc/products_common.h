@@ -1,0 +1,333 @@
+// What the grouped and 8-bit matrix products share: where a workgroup's tile lies among ragged groups, the
+// staging of operand tiles in LDS, the fragments read from it and the store of a result tile.  gfx950 only.
+//
+// Every product here is  D[m][n] = sum_k A[m][k] * B[n][k]  over operands that lie either with the
+// contraction contiguous (A[m][k] at m * ld + k) or across it (A[m][k] at k * ld + m, "TR"):
+//   forward         A = x  [row][k]   B = w [n][k]
+//   input gradient  A = dy [row][n]   B = w, contracted over its rows (TR)
+//   weight gradient A = dy, B = x, both contracted over their rows (TR, TR)
+// A stage holds 128 bytes of the contraction of every operand row: 128 8-bit, 64 bf16 or 32 fp32 elements.
+// MFMAs take B as their first operand, so that a lane's registers run along n, which is contiguous in
+// every result: 16-byte stores, and one activation scale per lane in the 8-bit product.
+#pragma once
+#include "c2d_common.h"
+#include "../../include/cap2det_products.h"
+#include <type_traits>
+
+namespace c2d_pr {
+namespace {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+typedef __attribute__((address_space(3))) void lds_void;
+
+constexpr unsigned OUTSIDE = 0x7FFFFF00u;  // an offset behind every buffer: the load returns zeros
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const void* p, long long bytes) {
+  const unsigned long long u = (unsigned long long)p;
+  const unsigned lo = __builtin_amdgcn_readfirstlane((unsigned)u);
+  const unsigned hi = __builtin_amdgcn_readfirstlane((unsigned)(u >> 32));
+  const unsigned nb = __builtin_amdgcn_readfirstlane(
+      (unsigned)(bytes < 0 ? 0 : bytes < (long long)OUTSIDE ? bytes : (long long)OUTSIDE));
+  return __builtin_amdgcn_make_buffer_rsrc((void*)(((unsigned long long)hi << 32) | lo), (short)0, (int)nb,
+                                           0x00020000);
+}
+
+// ---- ragged groups ------------------------------------------------------------------------------
+
+// Group boundaries as they are used: each offset clamped to [0, rows], and at least every earlier one.
+struct Span { int lo, hi; };
+
+// The spans of groups base .. base + 63, one per lane (empty behind the last group); `carry`: the
+// largest boundary so far, updated.
+__device__ __forceinline__ Span lane_span(const int* __restrict__ offsets, int groups, int rows, int base,
+                                          int* carry) {
+  const int i = base + (int)(threadIdx.x & 63);
+  int lo = max(0, min(rows, offsets[min(i, groups)]));
+  const int next = max(0, min(rows, offsets[min(i + 1, groups)]));
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int o = __shfl_up(lo, d, 64);
+    if ((int)(threadIdx.x & 63) >= d) lo = max(lo, o);
+  }
+  lo = max(lo, *carry);
+  const int hi = max(lo, next);
+  *carry = __builtin_amdgcn_readlane(hi, 63);
+  return {lo, i < groups ? hi : lo};
+}
+
+__device__ __forceinline__ int lane_prefix_sum(int v) {
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int o = __shfl_up(v, d, 64);
+    if ((int)(threadIdx.x & 63) >= d) v += o;
+  }
+  return v;
+}
+
+// One group's span (all waves, any lane).
+__device__ __forceinline__ Span group_span(const int* __restrict__ offsets, int groups, int rows, int e) {
+  int carry = 0;
+  for (int base = 0;; base += 64) {
+    const Span s = lane_span(offsets, groups, rows, base, &carry);
+    if (e < base + 64)
+      return {__builtin_amdgcn_readlane(s.lo, e - base), __builtin_amdgcn_readlane(s.hi, e - base)};
+  }
+}
+
+struct Place {
+  int e, lo, hi;   // the tile's group and its rows
+  int m0, nt;      // first row of the tile, column tile
+  bool live;       // false: the workgroup has no tile
+  int begin, end;  // rows outside [begin, end) are in no group
+  int spare, spares;  // a workgroup without a tile: its number among those that clear rows (-1: none)
+};
+
+// Tile of workgroup `bid` out of `nbid` (a multiple of 8).  The host cannot know how many row tiles the
+// groups make; it launches the largest number, rows / BM + groups, and each wave counts them here: one
+// or two loads and a dozen lane shuffles for 64 groups.  Workgroups go round the 8 XCDs by number; XCD x
+// takes the x-th eighth of the tiles, in bands of 4 row tiles by all column tiles, so that what
+// runs there at a time shares rows and weights in that XCD's L2.
+template <int BM>
+__device__ __forceinline__ Place place_tile(const int* __restrict__ offsets, int groups, int rows, int ntiles,
+                                            unsigned bid, unsigned nbid) {
+  Place p;
+  int mtiles = 0, carry = 0;
+  Span s = {0, rows};
+  int upto = 0;
+  if (!offsets) {
+    mtiles = (rows + BM - 1) / BM;
+    p.begin = 0;
+    p.end = rows;
+  } else {
+    for (int base = 0; base < groups; base += 64) {
+      s = lane_span(offsets, groups, rows, base, &carry);
+      if (base == 0) p.begin = __builtin_amdgcn_readlane(s.lo, 0);
+      upto = lane_prefix_sum((s.hi - s.lo + BM - 1) / BM);
+      mtiles += __builtin_amdgcn_readlane(upto, 63);
+    }
+    p.end = carry;
+  }
+  const int tiles = mtiles * ntiles;
+  const int xcd = bid & 7, local = bid >> 3, per = nbid >> 3;
+  const int q = tiles >> 3, r = tiles & 7;
+  const int count = q + (xcd < r ? 1 : 0);
+  p.live = local < count;
+  p.spares = 8 * (per - q - (r ? 1 : 0));
+  p.spare = -1;
+  if (!p.live) {
+    if (8 * (local - count) + xcd < p.spares) p.spare = 8 * (local - count) + xcd;
+    return p;
+  }
+  const int idx = xcd * q + min(xcd, r) + local;
+  constexpr int BAND = 4;
+  const int band = idx / (BAND * ntiles), at = idx - band * BAND * ntiles;
+  const int bm = min(BAND, mtiles - band * BAND);
+  const int mt = band * BAND + at % bm;
+  p.nt = at / bm;
+  if (!offsets) {
+    p.e = 0; p.lo = 0; p.hi = rows; p.m0 = mt * BM;
+    return p;
+  }
+  int before = 0;
+  if (groups > 64) carry = 0;
+  for (int base = 0;; base += 64) {
+    if (groups > 64) {
+      s = lane_span(offsets, groups, rows, base, &carry);
+      upto = lane_prefix_sum((s.hi - s.lo + BM - 1) / BM);
+    }
+    const unsigned long long has = __ballot(before + upto > mt);
+    if (has) {
+      const int l = __builtin_ctzll(has);
+      p.e = base + l;
+      p.lo = __builtin_amdgcn_readlane(s.lo, l);
+      p.hi = __builtin_amdgcn_readlane(s.hi, l);
+      const int mine = (p.hi - p.lo + BM - 1) / BM;
+      p.m0 = p.lo + (mt - (before + __builtin_amdgcn_readlane(upto, l) - mine)) * BM;
+      return p;
+    }
+    before += __builtin_amdgcn_readlane(upto, 63);
+  }
+}
+
+// The largest number of workgroups that place_tile can need, with some to spare that clear rows; 0: too many.
+inline unsigned place_grid(int BM, int groups, bool ragged, int rows, int ntiles) {
+  const long long mt = ragged ? (long long)rows / BM + (groups < rows ? groups : rows) : ((long long)rows + BM - 1) / BM;
+  const long long n = ((mt * ntiles + 7) / 8 + (ragged ? 8 : 0)) * 8;
+  return n < (1ll << 30) ? (unsigned)n : 0u;
+}
+
+// Rows in no group := 0, by the workgroups that have no tile.
+template <class T>
+__device__ __forceinline__ void clear_rest(const Place& p, T* y, long long ldy, int rows, int n, int threads) {
+  if (p.spare < 0) return;
+  const int rest = rows - (p.end - p.begin);
+  for (int i = p.spare; i < rest; i += p.spares) {
+    const int row = i < p.begin ? i : p.end + (i - p.begin);
+    for (int c = threadIdx.x; c < n; c += threads) y[row * ldy + c] = (T)0.0f;
+  }
+}
+
+// ---- staging --------------------------------------------------------------------------------------
+
+// One operand's tile of R rows (or, TR, R columns) by 128 bytes of the contraction, staged by NTH threads.
+//
+// LDS image, contraction contiguous: 128-byte rows, 16-byte chunk c of row r at c ^ ((r >> 1) & 7).  A
+// ds_read_b128 takes one chunk of 16 consecutive rows at a time; the XOR puts those on 16 different
+// 16-byte slots of the 256-byte bank period.  TR: 128 / ES rows of R * ES bytes as they lie in memory;
+// bf16 moves 64-byte granule g of row r to g ^ (r & 3), so that the four rows of a transposed read
+// (ds_read_b64_tr_b16) lie on four bank groups.  The image of a load to LDS is lane-linear: the XOR is
+// applied to the address that a lane fetches from.
+//
+// VEC: loads go to LDS directly (buffer_load ... lds, 16 bytes a lane), and lie outside their buffer, which
+// returns zeros, behind the operand's last row and behind the contraction's end.  Not VEC (a pitch, a
+// pointer or a length that 16-byte loads do not fit): element loads with their own bounds.
+template <int ES, bool TR, int R, int NTH, bool VEC>
+struct Tile {
+  static constexpr int BYTES = R * 128;
+  static constexpr int LOADS = BYTES / (NTH * 16);
+  static constexpr int EPC = 16 / ES;
+  static constexpr int KST = 128 / ES;               // contraction elements per stage
+  static constexpr int CPR = TR ? R * ES / 16 : 8;   // chunks per staged row
+  static constexpr int RPP = NTH / CPR;              // staged rows per pass
+  static_assert(LOADS * NTH * 16 == BYTES, "tile vs workgroup");
+  static_assert(NTH % CPR == 0 && (RPP % 16 == 0 || (TR && RPP % 4 == 0)), "the XOR is the same in every pass");
+
+  const char* base;
+  long long ld;          // bytes
+  int across, len;       // rows (TR: columns) from base that exist; contraction elements
+  int row, chunk;        // this thread's staged row and source chunk of the first pass
+  unsigned off[LOADS];
+  __amdgpu_buffer_rsrc_t rs;
+
+  __device__ __forceinline__ void begin(const void* p, long long ld_bytes, int across_, int len_) {
+    base = (const char*)p;
+    ld = ld_bytes;
+    across = min(across_, R);
+    len = len_;
+    row = threadIdx.x / CPR;
+    const int pos = threadIdx.x % CPR;
+    chunk = !TR ? pos ^ ((row >> 1) & 7) : ES == 2 ? pos ^ ((row & 3) << 2) : pos;
+    if (VEC) {
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) off[i] = (unsigned)((row + i * RPP) * (int)ld + chunk * 16);
+      if (!TR) rs = buffer_of(base, across > 0 ? (long long)(across - 1) * ld + (long long)len * ES : 0);
+    }
+  }
+
+  // stage `st` into LDS at `to`
+  __device__ __forceinline__ void issue(char* to, int st) {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if constexpr (VEC) {
+      if constexpr (TR) {
+        const long long k0 = (long long)st * KST;
+        const long long left = len - k0;
+        rs = buffer_of(base + k0 * ld, left > 0 && across > 0 ? (min(left, (long long)KST) - 1) * ld + (long long)across * ES : 0);
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i)
+          __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void*)(to + i * NTH * 16 + wave * 1024), 16, (int)off[i], 0, 0, 0);
+      } else {
+        const int k0 = st * KST;
+        const bool in = k0 + chunk * EPC < len;
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i)
+          __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void*)(to + i * NTH * 16 + wave * 1024), 16,
+                                                   (int)(in ? off[i] : OUTSIDE), k0 * ES, 0, 0);
+      }
+    } else {
+      typedef typename std::conditional<ES == 1, unsigned char,
+                                        typename std::conditional<ES == 2, unsigned short, unsigned>::type>::type elem_t;
+      typedef elem_t chunk_t __attribute__((ext_vector_type(EPC)));
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) {
+        const int r = row + i * RPP;
+        chunk_t v;
+#pragma unroll
+        for (int j = 0; j < EPC; ++j) {
+          const long long k = TR ? (long long)st * KST + r : (long long)st * KST + chunk * EPC + j;
+          const int a = TR ? chunk * EPC + j : r;
+          v[j] = 0;
+          if (k < len && a < across)
+            v[j] = *(const elem_t*)(base + (TR ? k * ld + (long long)a * ES : a * ld + k * ES));
+        }
+        *(chunk_t*)(to + i * NTH * 16 + threadIdx.x * 16) = v;
+      }
+    }
+  }
+};
+
+// All of this wave's loads to LDS have landed and its LDS reads are done; then the same of every wave.
+__device__ __forceinline__ void stage_barrier() {
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// ---- result -----------------------------------------------------------------------------------------
+
+__device__ __forceinline__ unsigned pack_bf16(float a, float b) {
+  bf16x2 v;
+  v[0] = (__bf16)a;
+  v[1] = (__bf16)b;
+  return __builtin_bit_cast(unsigned, v);
+}
+
+// A 32 x 32 result tile: lane l holds row m = l & 31, register r column 8 (r >> 2) + 4 (l >> 5) + (r & 3).
+// fp32: four 16-byte stores of 4 columns.  bf16: the halves of the wave exchange registers
+// (v_permlane32_swap) so that each holds 8 consecutive columns, two 16-byte stores.  `row`: this lane's row
+// of the result at the tile's first column, null if there is none; `cols`: columns that exist.
+template <bool BF16>
+__device__ __forceinline__ void store_tile(const f32x16& v, char* row, int cols, bool wide) {
+  const int lh = (threadIdx.x >> 5) & 1;
+  if constexpr (BF16) {
+    unsigned w[8];
+#pragma unroll
+    for (int g = 0; g < 8; ++g) w[g] = pack_bf16(v[2 * g], v[2 * g + 1]);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      // w[4h..4h+1]: columns 16h + 4 lh ..; w[4h+2..4h+3]: columns 16h + 8 + 4 lh ..
+      const auto x = __builtin_amdgcn_permlane32_swap(w[4 * h], w[4 * h + 2], false, false);
+      const auto y = __builtin_amdgcn_permlane32_swap(w[4 * h + 1], w[4 * h + 3], false, false);
+      const u32x4 o = {x[0], y[0], x[1], y[1]};  // columns 16 h + 8 lh .. + 7
+      const int c = 16 * h + 8 * lh;
+      if (row) {
+        if (wide && c + 8 <= cols) {
+          *(u32x4*)(row + c * 2) = o;
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (c + j < cols) ((unsigned short*)row)[c + j] = (unsigned short)(o[j >> 1] >> (16 * (j & 1)));
+        }
+      }
+    }
+  } else {
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int c = 8 * g + 4 * lh;
+      if (row) {
+        if (wide && c + 4 <= cols) {
+          *(f32x4*)(row + c * 4) = f32x4{v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]};
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (c + j < cols) ((float*)row)[c + j] = v[4 * g + j];
+        }
+      }
+    }
+  }
+}
+
+inline bool aligned16(const void* p, long long pitch_bytes) {
+  return ((unsigned long long)p & 15) == 0 && (pitch_bytes & 15) == 0;
+}
+
+}  // namespace
+}  // namespace c2d_pr

@@ -831,3 +831,230 @@ def x9_planes(t):
   split3_bf16(t.view(-1), planes)
   f32x9_bind(t.view(-1), planes)
   return planes
+
+
+# -- grouped and 8-bit matrix products (include/cap2det_products.h) -------------------------------
+#
+# Groups of rows are given by `offsets`, an int32 device tensor of groups + 1 row numbers: group e owns
+# the rows offsets[e] .. offsets[e + 1] - 1 and may be empty.  Nothing here reads them on the host.  An offset
+# outside [0, rows] counts as the nearer end, one below an earlier one as that one.  Rows in no group are
+# not read; in a result they are zero, or, where `out` is given, left as they were.
+#
+# Matrices may be row-strided views (columns contiguous).  Everything is queued on the current stream of the
+# current device, where the tensors have to be; results and workspaces of one call are the call's own, so
+# that calls on several streams and captured graphs share none.  A step plan holds addresses: hand it `out`.
+
+FP8_BLOCK = 128
+FP8_TYPES = (torch.float8_e4m3fn, torch.float8_e5m2)
+_PRODUCT_TYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float8_e4m3fn: 2, torch.float8_e5m2: 3}
+
+
+def _need(ok, what):
+  if not ok:
+    raise ValueError(what)
+
+
+def _on_device(t, name):
+  _need(t.is_cuda, "%s: a device tensor is wanted, got one on %s" % (name, t.device))
+  _need(t.device.index == torch.cuda.current_device(),
+        "%s: on %s, but the current device is cuda:%d" % (name, t.device, torch.cuda.current_device()))
+
+
+def _device_tensor(t, name, dtypes, dims):
+  _need(isinstance(t, torch.Tensor), "%s: a tensor is wanted, got %s" % (name, type(t).__name__))
+  _on_device(t, name)
+  _need(t.dtype in dtypes, "%s: one of %s is wanted, got %s" % (name, ", ".join(map(str, dtypes)), t.dtype))
+  _need(t.dim() in dims, "%s: %s dimensions are wanted, got shape %s" % (name, " or ".join(map(str, dims)),
+                                                                       tuple(t.shape)))
+  return t
+
+
+def _pitch(t, name):
+  """Row pitch of a matrix in elements; columns have to be contiguous and rows apart."""
+  rows, cols = t.shape
+  if rows == 0 or cols == 0:
+    return max(cols, 1)
+  _need(cols == 1 or t.stride(1) == 1, "%s: columns have to be contiguous, got strides %s" % (name, t.stride()))
+  if rows == 1:
+    return cols
+  _need(t.stride(0) >= cols, "%s: rows overlap, got strides %s of shape %s" % (name, t.stride(), tuple(t.shape)))
+  return t.stride(0)
+
+
+def _whole(t, name):
+  _need(t.is_contiguous(), "%s: has to be contiguous, got strides %s of shape %s" % (name, t.stride(), tuple(t.shape)))
+  return t
+
+
+def _group_offsets(offsets, groups):
+  _device_tensor(offsets, "offsets", (torch.int32,), (1,))
+  _need(offsets.numel() == groups + 1, "offsets: %d numbers are wanted for %d groups, got %d"
+        % (groups + 1, groups, offsets.numel()))
+  return _whole(offsets, "offsets")
+
+
+def _result(out, shape, dtypes, dtype, device, *inputs):
+  """(result tensor, whether rows in no group are to be cleared)."""
+  if out is None:
+    return torch.empty(shape, dtype=dtype, device=device), True
+  _device_tensor(out, "out", dtypes, (len(shape),))
+  _need(tuple(out.shape) == tuple(shape), "out: shape %s is wanted, got %s" % (tuple(shape), tuple(out.shape)))
+  lo, hi = _extent(out)
+  for t in inputs:
+    a, b = _extent(t)
+    _need(hi <= a or b <= lo, "out: shares memory with an operand")
+  return out, False
+
+
+def _extent(t):
+  """First and last + 1 byte that a tensor reaches."""
+  if t is None or t.numel() == 0:
+    return 0, 0
+  last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+  return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+
+def _workspace(nbytes, device):
+  ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+  return ws, (None if ws is None else ws.data_ptr()), nbytes
+
+
+def fp8_quantize(x, block_rows=1, dtype=torch.float8_e4m3fn):
+  """8-bit values and fp32 scales of a matrix, or of a stack of matrices: x [.., rows, cols] fp32 or bf16 ->
+  (q [.., rows, cols], scale [.., ceil(rows / block_rows), ceil(cols / 128)]), x ~ q * scale of its block.
+
+  Blocks are block_rows x 128: 1 for activations, 128 for weights.  scale = max |x| / F, at least
+  2^-126, F = 448 (float8_e4m3fn) or 57344 (float8_e5m2); q = x / scale in fp32, to the nearest, ties to
+  even.  A NaN stays one and takes no part in the maximum, an infinity makes its block's values NaN.
+  The blocks of a weight matrix w are square: q.t().contiguous() and scale.t().contiguous() are w.t()'s."""
+  _device_tensor(x, "x", (torch.float32, torch.bfloat16), (2, 3))
+  _need(dtype in FP8_TYPES, "dtype: one of %s is wanted, got %s" % (", ".join(map(str, FP8_TYPES)), dtype))
+  _need(block_rows in (1, FP8_BLOCK), "block_rows: 1 or %d, got %r" % (FP8_BLOCK, block_rows))
+  batch, (rows, cols) = (1 if x.dim() == 2 else x.shape[0]), x.shape[-2:]
+  lead = tuple(x.shape[:-2])
+  q = torch.empty(lead + (rows, cols), dtype=dtype, device=x.device)
+  scale = torch.empty(lead + (-(-rows // block_rows), -(-cols // FP8_BLOCK)), device=x.device)
+  if q.numel() == 0:
+    return q, scale
+  ld = _pitch(x if x.dim() == 2 else x[0], "x")
+  _lib.call("c2dp_fp8_quantize", x.data_ptr(), _PRODUCT_TYPE[x.dtype], ld, x.stride(0) if x.dim() == 3 else 0,
+            q.data_ptr(), _PRODUCT_TYPE[dtype], scale.data_ptr(), batch, rows, cols, block_rows, _stream())
+  return q, scale
+
+
+def _fp8_product(a, a_scale, b, b_scale, offsets, out, out_dtype, bias, relu):
+  groups, n, k = b.shape
+  rows = a.shape[0]
+  _need(a.shape[1] == k, "a: %d columns are wanted, got shape %s" % (k, tuple(a.shape)))
+  kb, nb = -(-k // FP8_BLOCK), -(-n // FP8_BLOCK)
+  _need(tuple(a_scale.shape) == (rows, kb), "a_scale: shape %s is wanted, got %s" % ((rows, kb), tuple(a_scale.shape)))
+  _need(b_scale.numel() == groups * nb * kb and tuple(b_scale.shape[-2:]) == (nb, kb),
+        "b_scale: shape %s is wanted, got %s" % ((groups, nb, kb), tuple(b_scale.shape)))
+  for t, name in ((a_scale, "a_scale"), (b, "b"), (b_scale, "b_scale")):
+    _whole(t, name)
+  if bias is not None:
+    _need(bias.numel() == groups * n and bias.shape[-1] == n, "bias: shape %s is wanted, got %s"
+          % ((groups, n), tuple(bias.shape)))
+    _whole(bias, "bias")
+  _need(out is not None or out_dtype in (torch.bfloat16, torch.float32),
+        "out_dtype: torch.bfloat16 or torch.float32, got %s" % (out_dtype,))
+  y, clear = _result(out, (rows, n), (torch.bfloat16, torch.float32), out_dtype, a.device, a, a_scale, b, b_scale,
+                     bias, offsets)
+  if y.numel() == 0:
+    return y
+  ws, ws_ptr, ws_bytes = _workspace(int(_lib.load().c2dp_fp8_matmul_workspace_bytes(groups, rows, n, k)), a.device)
+  _lib.call("c2dp_fp8_matmul", a.data_ptr(), _PRODUCT_TYPE[a.dtype], _pitch(a, "a"), a_scale.data_ptr(), b.data_ptr(),
+            b_scale.data_ptr(), None if offsets is None else offsets.data_ptr(), groups,
+            None if bias is None else bias.data_ptr(), int(bool(relu)), y.data_ptr(), _PRODUCT_TYPE[y.dtype],
+            _pitch(y, "out"), rows, n, k, int(clear), ws_ptr, ws_bytes, _stream())
+  return y
+
+
+def fp8_matmul(a, a_scale, b, b_scale, out=None, out_dtype=torch.bfloat16, bias=None, relu=False):
+  """act(a . b^T + bias) of block-scaled 8-bit matrices with fp32 sums: a [rows, k] with a_scale
+  [rows, ceil(k / 128)] (fp8_quantize, block_rows 1; float8_e4m3fn, or float8_e5m2 as gradients use), b
+  [n, k] float8_e4m3fn with b_scale [ceil(n / 128), ceil(k / 128)] (block_rows 128), bias [n] fp32 ->
+  [rows, n] bf16 or fp32.  The input gradient is the same product on the transposed weight."""
+  _device_tensor(a, "a", FP8_TYPES, (2,))
+  _device_tensor(a_scale, "a_scale", (torch.float32,), (2,))
+  _device_tensor(b, "b", FP8_TYPES[:1], (2,))
+  _device_tensor(b_scale, "b_scale", (torch.float32,), (2,))
+  if bias is not None:
+    _device_tensor(bias, "bias", (torch.float32,), (1,))
+  return _fp8_product(a, a_scale, b.unsqueeze(0), b_scale, None, out, out_dtype, bias, relu)
+
+
+def grouped_matmul_fp8(a, a_scale, b, b_scale, offsets, out=None, out_dtype=torch.bfloat16, bias=None, relu=False):
+  """fp8_matmul with one weight matrix per group of rows: b [groups, n, k], b_scale [groups, ceil(n / 128),
+  ceil(k / 128)], bias [groups, n]."""
+  _device_tensor(a, "a", FP8_TYPES, (2,))
+  _device_tensor(a_scale, "a_scale", (torch.float32,), (2,))
+  _device_tensor(b, "b", FP8_TYPES[:1], (3,))
+  _device_tensor(b_scale, "b_scale", (torch.float32,), (3,))
+  if bias is not None:
+    _device_tensor(bias, "bias", (torch.float32,), (2,))
+  _need(b.shape[0] > 0, "b: at least one group is wanted, got shape %s" % (tuple(b.shape),))
+  return _fp8_product(a, a_scale, b, b_scale, _group_offsets(offsets, b.shape[0]), out, out_dtype, bias, relu)
+
+
+def _grouped_rows(name, x, w, offsets, out, out_dtype, n, k, result_cols, x_cols, x_name):
+  types = (torch.float32, torch.bfloat16)
+  _device_tensor(x, x_name, types, (2,))
+  _need(w.dtype == x.dtype, "w: %s as %s is wanted, got %s" % (x.dtype, x_name, w.dtype))
+  _need(x.shape[1] == x_cols, "%s: %d columns are wanted, got shape %s" % (x_name, x_cols, tuple(x.shape)))
+  _whole(w, "w")
+  _group_offsets(offsets, w.shape[0])
+  out_dtype = out_dtype or x.dtype
+  allowed = (torch.float32,) if x.dtype == torch.float32 else types
+  _need(out_dtype in allowed, "out_dtype: one of %s is wanted, got %s" % (", ".join(map(str, allowed)), out_dtype))
+  rows = x.shape[0]
+  y, clear = _result(out, (rows, result_cols), allowed, out_dtype, x.device, x, w, offsets)
+  if y.numel() == 0:
+    return y
+  _lib.call(name, x.data_ptr(), _PRODUCT_TYPE[x.dtype], _pitch(x, x_name), w.data_ptr(), offsets.data_ptr(), w.shape[0],
+            y.data_ptr(), _PRODUCT_TYPE[y.dtype], _pitch(y, "out"), rows, n, k, int(clear), _stream())
+  return y
+
+
+def _group_weights(w):
+  _device_tensor(w, "w", (torch.float32, torch.bfloat16), (3,))
+  _need(w.shape[0] > 0, "w: at least one group is wanted, got shape %s" % (tuple(w.shape),))
+  return w.shape
+
+
+def grouped_matmul(x, w, offsets, out=None, out_dtype=None):
+  """x_e . w_e^T for every group e of rows: x [rows, k], w [groups, n, k], both fp32 or both bf16 -> [rows, n] of
+  x's type (bf16 operands: or fp32, by out_dtype or by `out`); fp32 sums."""
+  _, n, k = _group_weights(w)
+  return _grouped_rows("c2dp_grouped_matmul", x, w, offsets, out, out_dtype, n, k, n, k, "x")
+
+
+def grouped_matmul_dgrad(dy, w, offsets, out=None, out_dtype=None):
+  """Input gradient of grouped_matmul: dy [rows, n], w [groups, n, k] -> dx [rows, k] = dy_e . w_e."""
+  _, n, k = _group_weights(w)
+  return _grouped_rows("c2dp_grouped_matmul_dgrad", dy, w, offsets, out, out_dtype, n, k, k, n, "dy")
+
+
+def grouped_matmul_wgrad(x, dy, offsets, out=None, accumulate=False):
+  """Weight gradient of grouped_matmul: x [rows, k], dy [rows, n] -> dw [groups, n, k] fp32, dw_e =
+  dy_e^T . x_e, zero for an empty group; accumulate=True adds that to `out`.  The same call gives the same
+  bits."""
+  types = (torch.float32, torch.bfloat16)
+  _device_tensor(x, "x", types, (2,))
+  _device_tensor(dy, "dy", (x.dtype,), (2,))
+  _need(dy.shape[0] == x.shape[0], "dy: %d rows are wanted, got shape %s" % (x.shape[0], tuple(dy.shape)))
+  _device_tensor(offsets, "offsets", (torch.int32,), (1,))
+  groups, rows, n, k = offsets.numel() - 1, x.shape[0], dy.shape[1], x.shape[1]
+  _need(groups > 0, "offsets: at least two numbers are wanted, got %d" % offsets.numel())
+  _group_offsets(offsets, groups)
+  _need(out is not None or not accumulate, "accumulate: there is no `out` to add to")
+  dw, _ = _result(out, (groups, n, k), (torch.float32,), torch.float32, x.device, x, dy, offsets)
+  _whole(dw, "out")
+  if dw.numel() == 0:
+    return dw
+  ws, ws_ptr, ws_bytes = _workspace(
+      int(_lib.load().c2dp_grouped_matmul_wgrad_workspace_bytes(groups, rows, n, k)), x.device)
+  _lib.call("c2dp_grouped_matmul_wgrad", x.data_ptr(), _PRODUCT_TYPE[x.dtype], _pitch(x, "x"), dy.data_ptr(),
+            _pitch(dy, "dy"), offsets.data_ptr(), groups, dw.data_ptr(), rows, n, k,
+            int(bool(accumulate)), ws_ptr, ws_bytes, _stream())
+  return dw

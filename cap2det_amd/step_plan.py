@@ -128,7 +128,7 @@ class StepPlan(object):
     self.handle = ctypes.c_void_p(self.lib.c2d_plan_create())
     if not self.handle.value:
       raise MemoryError("c2d_plan_create")
-    self.sigs = _lib.header_signatures()
+    self.sigs = dict(_lib.header_signatures(), **_lib.product_signatures())
     self.keep = []                 # host arrays / structs whose addresses the plan holds
     self.ranges = []               # (lo, hi, slot) of the bound tensors
     self.slot_names = []           # slot -> name

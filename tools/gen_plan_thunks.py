@@ -1,21 +1,21 @@
-"""Generates cap2det_amd/csrc/plan_thunks.inc from include/cap2det_hip.h: one typed thunk per C-ABI
+"""Generates cap2det_amd/csrc/plan_thunks.inc from the headers under include/: one typed thunk per C-ABI
 entry point, `int thunk(const long long* v)`, that unpacks the recorded argument words into the
 entry point's own parameter types (pointers and integers from the 64-bit word, floats from its low
 32 bits) — the step plan of csrc/plan.hip calls entry points through these, never through a guessed
 calling convention.  Run by the Makefile; the output is not committed.
 
-  python tools/gen_plan_thunks.py include/cap2det_hip.h cap2det_amd/csrc/plan_thunks.inc
+  python tools/gen_plan_thunks.py include/cap2det_hip.h include/cap2det_products.h cap2det_amd/csrc/plan_thunks.inc
 """
 import re
 import sys
 
 
 def main():
-  header, out = sys.argv[1], sys.argv[2]
-  text = re.sub(r"/\*.*?\*/", "", open(header).read(), flags=re.S)
-  lines = ["// GENERATED by tools/gen_plan_thunks.py from include/cap2det_hip.h — do not edit.", ""]
+  headers, out = sys.argv[1:-1], sys.argv[-1]
+  text = re.sub(r"/\*.*?\*/", "", "\n".join(open(h).read() for h in headers), flags=re.S)
+  lines = ["// GENERATED by tools/gen_plan_thunks.py from the headers under include/ — do not edit.", ""]
   table = []
-  for m in re.finditer(r"(const char\*|unsigned long long|unsigned int|long long|int)\s+(c2d_\w+)"
+  for m in re.finditer(r"(const char\*|unsigned long long|unsigned int|long long|int)\s+(c2dp?_\w+)"
                        r"\s*\(([^)]*)\)\s*;", text):
     ret, name, params = m.group(1), m.group(2), m.group(3).strip()
     if ret != "int" or name.startswith("c2d_plan_"):
