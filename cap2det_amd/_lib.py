@@ -123,7 +123,9 @@ recorder_thread = None      # only calls of the thread that records belong to th
 
 def call(name, *args):
   """Calls C-ABI function `name`; raises Cap2DetHipError on a non-zero return."""
-  check(getattr(load(), name)(*args), name)
+  code = getattr(_lib or load(), name)(*args)
+  if code != 0:
+    check(code, name)
   if recorder is not None and threading.get_ident() == recorder_thread:
     recorder.add_call(name, args)
 

@@ -1,6 +1,6 @@
 // 8-bit floating-point storage: the block quantiser and the product of block-scaled matrices, for one
 // weight matrix or one per group of rows.
-#include "products_common.h"
+#include "products_few.h"
 
 using namespace c2d_pr;
 
@@ -13,24 +13,25 @@ namespace {
 // rounded too): three operations an element where a division takes ten, and no value near a tie falls on
 // another side than the true quotient's.  |x| <= F * scale up to rounding, so nothing overflows the type.
 
-template <class T>
-struct Eight { f32x4 lo, hi; };
-
+// (any address)
 __device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
-  const f32x4 a = *(const f32x4*)p, b = *(const f32x4*)(p + 4);
+  f32x4 a, b;
+  __builtin_memcpy(&a, p, 16);
+  __builtin_memcpy(&b, p + 4, 16);
 #pragma unroll
   for (int j = 0; j < 4; ++j) { v[j] = a[j]; v[4 + j] = b[j]; }
 }
 __device__ __forceinline__ void load8(const __bf16* p, float (&v)[8]) {
-  const bf16x8 a = *(const bf16x8*)p;
+  bf16x8 a;
+  __builtin_memcpy(&a, p, 16);
 #pragma unroll
   for (int j = 0; j < 8; ++j) v[j] = (float)a[j];
 }
 
 // eight elements of a row from column c, zeros behind the last
 template <class T>
-__device__ __forceinline__ void load_chunk(const T* row, int c, int cols, bool wide, float (&v)[8]) {
-  if (wide && c + 8 <= cols) {
+__device__ __forceinline__ void load_chunk(const T* row, int c, int cols, float (&v)[8]) {
+  if (c + 8 <= cols) {
     load8(row + c, v);
   } else {
 #pragma unroll
@@ -81,9 +82,9 @@ __device__ __forceinline__ u32x2 quantize8(const float (&v)[8], float scale) {
   return o;
 }
 
-__device__ __forceinline__ void store_chunk(unsigned char* row, int c, int cols, bool wide, u32x2 q) {
-  if (wide && c + 8 <= cols) {
-    *(u32x2*)(row + c) = q;
+__device__ __forceinline__ void store_chunk(unsigned char* row, int c, int cols, u32x2 q) {
+  if (c + 8 <= cols) {
+    store_at((char*)row + c, q);
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j)
@@ -98,7 +99,6 @@ struct QuantArgs {
   float* scale;
   int rows, cols, kb, per_wg;  // per_wg: rows of a workgroup (1 x 128 blocks)
   unsigned magic;              // ceil(2^32 / kb): t / kb = umulhi(t, magic) for t < 2^16
-  int wide_in, wide_out;
 };
 
 // Blocks of 1 x 128: 16 lanes a block, 8 elements a lane, up to 64 blocks a workgroup, all of whose loads
@@ -118,7 +118,7 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(QuantArgs a) {
     if (t < tasks) {
       const int r = a.kb > 64 || a.kb == 1 ? (a.kb == 1 ? t : 0) : (int)__umulhi((unsigned)t, a.magic);
       const int j = a.kb > 64 ? j0 + t : t - r * a.kb;
-      load_chunk(x + (row0 + r) * a.ldx, j * 128 + lane16 * 8, a.cols, a.wide_in, v[u]);
+      load_chunk(x + (row0 + r) * a.ldx, j * 128 + lane16 * 8, a.cols, v[u]);
     }
   }
 #pragma unroll
@@ -129,7 +129,7 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(QuantArgs a) {
       const int j = a.kb > 64 ? j0 + t : t - r * a.kb;
       const float s = scale_of<E5M2>(largest_of_16_lanes(largest(v[u])));
       const long long row = (long long)blockIdx.z * a.rows + row0 + r;
-      store_chunk(a.q + row * a.cols, j * 128 + lane16 * 8, a.cols, a.wide_out, quantize8<E5M2>(v[u], s));
+      store_chunk(a.q + row * a.cols, j * 128 + lane16 * 8, a.cols, quantize8<E5M2>(v[u], s));
       if (lane16 == 0) a.scale[row * a.kb + j] = s;
     }
   }
@@ -149,7 +149,7 @@ __global__ __launch_bounds__(256) void quantize_square_kernel(QuantArgs a) {
   for (int u = 0; u < 8; ++u) {
     const int r = bi * 128 + slot + 16 * u;
     if (r < a.rows) {
-      load_chunk(x + r * a.ldx, c, a.cols, a.wide_in, v[u]);
+      load_chunk(x + r * a.ldx, c, a.cols, v[u]);
     } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[u][j] = 0.0f;
@@ -165,7 +165,7 @@ __global__ __launch_bounds__(256) void quantize_square_kernel(QuantArgs a) {
   for (int u = 0; u < 8; ++u) {
     const int r = bi * 128 + slot + 16 * u;
     if (r < a.rows)
-      store_chunk(a.q + ((long long)blockIdx.y * a.rows + r) * a.cols, c, a.cols, a.wide_out, quantize8<E5M2>(v[u], s));
+      store_chunk(a.q + ((long long)blockIdx.y * a.rows + r) * a.cols, c, a.cols, quantize8<E5M2>(v[u], s));
   }
   if (threadIdx.x == 0) a.scale[((long long)blockIdx.y * mb + bi) * a.kb + bj] = s;
 }
@@ -207,8 +207,6 @@ extern "C" int c2dp_fp8_quantize(const void* x, int x_type, long long ldx, long 
   a.per_wg = 0;
   a.magic = (unsigned)((0x100000000ull + a.kb - 1) / a.kb);
   const int es = x_type == C2DP_F32 ? 4 : 2;
-  a.wide_in = aligned16(x, ldx * es) && (batch == 1 || x_batch * es % 16 == 0);
-  a.wide_out = cols % 8 == 0 && ((unsigned long long)q & 7) == 0;
   const hipStream_t s = (hipStream_t)stream;
   if (es == 4)
     return q_type == C2DP_E5M2 ? launch_quantize<float, true>(a, batch, block_rows, s)
@@ -220,69 +218,87 @@ extern "C" int c2dp_fp8_quantize(const void* x, int x_type, long long ldx, long 
 // ---- product ----------------------------------------------------------------------------------------
 //
 // y = act(sum_c a_scale[.][c] b_scale[.][c] (a_c . b_c) + bias), c the blocks of 128 k.  A stage of the
-// operand tiles is one block c: two v_mfma_f32_32x32x64_f8f6f4 from zero, then one multiply-add per sum with
-// the block's scale.  A lane's sums lie in ONE row of the result (products_common.h), so that
-// the scale is one number per lane and tile.
+// operand tiles is one block c: its products are summed from zero, then one multiply-add per sum with the
+// block's scale.  A lane's sums lie in ONE row of the result (products_common.h), so that the scale is one
+// number per lane and tile.
+//
+// The 8-bit matrix instructions add their products with fewer bits than fp32 holds (every shape of them:
+// 1.4e-5 relative to a block's sum for normal values, measured).  A bf16 result, which is rounded to 2^-9, takes
+// them.  For an fp32 result the fragments are widened to bf16, which holds every 8-bit value exactly, and
+// go through the bf16 matrix instructions, whose sums are fp32 (2e-7), at half the rate.
 
 namespace {
 
-struct Fp8Args {
-  const char* a;
-  long long lda;
-  const float* a_scale;
-  const char* b;
-  const float* b_scale;
-  const int* offsets;
-  const float* bias;
-  char* y;
-  long long ldy;
-  int groups, rows, n, k, kb, nb;
-  int ntiles, wide, clear, relu;
-};
-
-// 32 rows from r0, 64 k of step s: chunks 4 s + 2 lh, + 1
-__device__ __forceinline__ i32x8 fp8_frag(const char* t, int r0, int s) {
+// 32 rows from r0 of a stage: chunks 2 c + lh, c = C0 .. C1 - 1, of a lane's row
+template <int C0, int C1>
+__device__ __forceinline__ void fp8_load(const char* t, int r0, i32x4 (&f)[4]) {
   const int lane = threadIdx.x & 63, li = lane & 31, lh = lane >> 5;
   const char* p = t + (r0 + li) * 128;
   const int x = (li >> 1) & 7;
-  const i32x4 lo = *(const i32x4*)(p + (((4 * s + 2 * lh) ^ x) << 4));
-  const i32x4 hi = *(const i32x4*)(p + (((4 * s + 2 * lh + 1) ^ x) << 4));
-  return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+  for (int c = C0; c < C1; ++c) f[c] = *(const i32x4*)(p + (((2 * c + lh) ^ x) << 4));
 }
 
-template <bool E5M2>
-__device__ __forceinline__ f32x16 fp8_mfma(i32x8 b, i32x8 a, f32x16 c) {
-  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(b, a, c, 0, E5M2 ? 1 : 0, 0, 0, 0, 0);
+// half a stage's products (64 k) of 32 columns and 32 rows, added to z
+template <bool E5M2, bool WIDE>
+__device__ __forceinline__ f32x16 fp8_half(const i32x4 (&b)[4], const i32x4 (&a)[4], int h, f32x16 z) {
+  if constexpr (WIDE) {
+#pragma unroll
+    for (int c = 2 * h; c < 2 * h + 2; ++c) {
+      z = __builtin_amdgcn_mfma_f32_32x32x16_bf16(widen8<false>(b[c][0], b[c][1]), widen8<E5M2>(a[c][0], a[c][1]), z, 0, 0, 0);
+      z = __builtin_amdgcn_mfma_f32_32x32x16_bf16(widen8<false>(b[c][2], b[c][3]), widen8<E5M2>(a[c][2], a[c][3]), z, 0, 0, 0);
+    }
+    return z;
+  } else {
+    return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
+        __builtin_shufflevector(b[2 * h], b[2 * h + 1], 0, 1, 2, 3, 4, 5, 6, 7),
+        __builtin_shufflevector(a[2 * h], a[2 * h + 1], 0, 1, 2, 3, 4, 5, 6, 7), z, 0, E5M2 ? 1 : 0, 0, 0, 0, 0);
+  }
 }
 
-template <bool E5M2, int WM, int WN, int MT, int NT, bool VEC, bool OUT16>
-__global__ __launch_bounds__(WM * WN * 64) void fp8_tile_kernel(Fp8Args a) {
-  constexpr int BM = WM * MT * 32, BN = WN * NT * 32, NTH = WM * WN * 64;
+// The stages of B go round DB buffers, those of A round DB + 1: while a stage is multiplied, the next of B and
+// the next two of A are on their way (DB = 2).  Within a stage the loads are issued between the matrix
+// instructions of its first tiles, and a tile's scaling runs under the matrix instructions of the next.
+//
+// KG > 1: KG groups of WM x WN waves share the tile, group g taking the stages g, g + KG, ..; their sums are
+// joined through LDS, in the groups' order.  A stage of a small tile is a chain of waits (barrier, LDS read, two
+// matrix instructions, scaling) of 0.5 us whatever its size (64 x 64 tiles): where there is a workgroup per CU
+// or less, KG chains run side by side (256 x 4096 x 4096: 17.6 us, with two groups 13.6, with four 14.6).
+template <bool E5M2, int WM, int WN, int MT, int NT, int KG, int DB, bool VEC, bool OUT16>
+__global__ __launch_bounds__(WM * WN * KG * 64, 2) void fp8_tile_kernel(FewArgs a) {
+  constexpr int BM = WM * MT * 32, BN = WN * NT * 32, NTH = WM * WN * 64, DA = DB + 1, TILES = MT * NT;
   typedef Tile<1, false, BM, NTH, VEC> TA;
   typedef Tile<1, false, BN, NTH, VEC> TB;
-  constexpr int STAGE = TA::BYTES + TB::BYTES;
-  static_assert(NT * 32 <= 128, "a wave's columns share a block of b");
-  __shared__ __attribute__((aligned(1024))) char smem[2 * STAGE];
+  constexpr int PASSES = TA::LOADS + TB::LOADS;
+  constexpr int RING = DA * TA::BYTES + DB * TB::BYTES;
+  static_assert(128 % (NT * 32) == 0, "a wave's columns share a block of b");
+  static_assert(KG == 1 || (KG - 1) * NTH * 64 <= KG * RING, "the sums are joined a tile at a time in the ring's LDS");
+  __shared__ __attribute__((aligned(1024))) char smem[KG * RING];
   typedef typename std::conditional<OUT16, __bf16, float>::type out_t;
   const Place p = place_tile<BM>(a.offsets, a.groups, a.rows, a.ntiles, blockIdx.x, gridDim.x);
   if (!p.live) {
-    if (a.clear) clear_rest(p, (out_t*)a.y, a.ldy, a.rows, a.n, NTH);
+    if (a.clear) clear_rest(p, (out_t*)a.y, a.ldy, a.rows, a.n, NTH * KG);
     return;
   }
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int group = KG == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / NTH), tid = threadIdx.x - group * NTH;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / WN, wn = wave % WN;
   const int lane = threadIdx.x & 63, li = lane & 31, lh = lane >> 5;
   const int n0 = p.nt * BN;
+  char* const ring_a = smem + group * RING;
+  char* const ring_b = ring_a + DA * TA::BYTES;
   TA ta;
   TB tb;
-  ta.begin(a.a + (long long)p.m0 * a.lda, a.lda, p.hi - p.m0, a.k);
-  tb.begin(a.b + ((long long)p.e * a.n + n0) * a.k, a.k, a.n - n0, a.k);
+  ta.begin(a.a + (long long)p.m0 * a.lda, a.lda, p.hi - p.m0, a.k, tid);
+  tb.begin(a.b + p.e * a.b_group + n0 * a.ldb, a.ldb, a.n - n0, a.k, tid);
   // scales: one row each for this lane's MT rows, one block of columns for the wave
-  const float* as[MT];
+  const float* const as = a.a_scale + (long long)p.m0 * a.kb;
+  unsigned as_at[MT];
 #pragma unroll
-  for (int i = 0; i < MT; ++i)
-    as[i] = a.a_scale + (long long)min(p.m0 + (wm * MT + i) * 32 + li, p.hi - 1) * a.kb;
-  const float* const bs = a.b_scale + ((long long)p.e * a.nb + min((n0 + wn * NT * 32) >> 7, a.nb - 1)) * a.kb;
+  for (int i = 0; i < MT; ++i) as_at[i] = (unsigned)(min((wm * MT + i) * 32 + li, p.hi - 1 - p.m0) * a.kb);
+  typedef __attribute__((address_space(4))) const float scalar_float;
+  const scalar_float* const bs = (const scalar_float*)(unsigned long long)(
+      a.b_scale + ((long long)p.e * a.nb + min((n0 + wn * NT * 32) >> 7, a.nb - 1)) * a.kb);
 
   f32x16 acc[MT][NT];
 #pragma unroll
@@ -291,45 +307,104 @@ __global__ __launch_bounds__(WM * WN * 64) void fp8_tile_kernel(Fp8Args a) {
     for (int j = 0; j < NT; ++j)
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
-  float scale[MT];
-  if (a.kb > 0) {
-    ta.issue(smem, 0);
-    tb.issue(smem + TA::BYTES, 0);
+  const int rounds = (a.kb + KG - 1) / KG;
+  float row_scale[MT], col_scale = 0.0f;
+  // (a stage behind the last is zeros that nobody reads, or that count nothing: its scale is zero)
+  auto load_scales = [&](int st) {
+    const int c = min(st, a.kb - 1);
+    col_scale = st < a.kb ? bs[c] : 0.0f;
 #pragma unroll
-    for (int i = 0; i < MT; ++i) scale[i] = as[i][0] * bs[0];
-  }
-  for (int it = 0; it < a.kb; ++it) {
-    char* const now = smem + (it & 1) * STAGE;
-    char* const next = smem + (~it & 1) * STAGE;
-    float s_now[MT];
+    for (int i = 0; i < MT; ++i) row_scale[i] = as[as_at[i] + (unsigned)c];
+  };
+  if (rounds > 0) {
+    load_scales(group);
+    ta.issue(ring_a, group);
 #pragma unroll
-    for (int i = 0; i < MT; ++i) s_now[i] = scale[i];
-    stage_barrier();
-    if (it + 1 < a.kb) {
-      ta.issue(next, it + 1);
-      tb.issue(next + TA::BYTES, it + 1);
-#pragma unroll
-      for (int i = 0; i < MT; ++i) scale[i] = as[i][it + 1] * bs[it + 1];
+    for (int d = 0; d < DB - 1; ++d) {
+      tb.issue(ring_b + d * TB::BYTES, d * KG + group);
+      ta.issue(ring_a + (d + 1) * TA::BYTES, (d + 1) * KG + group);
     }
-    const char* const sa = now + wm * MT * 32 * 128;
-    const char* const sb = now + TA::BYTES + wn * NT * 32 * 128;
-    i32x8 fb[NT][2];
+  }
+  int now_a = 0, now_b = 0, next_a = DA - 1, next_b = DB - 1;
+  for (int it = 0; it < rounds; ++it) {
+    // (behind this stage's B have been issued: A of the next, and DB - 2 whole stages)
+    stage_barrier<VEC, TA::LOADS + (DB - 2) * PASSES>();
+    float scale[MT];
 #pragma unroll
-    for (int j = 0; j < NT; ++j) { fb[j][0] = fp8_frag(sb, j * 32, 0); fb[j][1] = fp8_frag(sb, j * 32, 1); }
+    for (int i = 0; i < MT; ++i) scale[i] = KG > 1 && col_scale == 0.0f ? 0.0f : row_scale[i] * col_scale;
+    load_scales((it + 1) * KG + group);  // in front of the loads to LDS
+    const int st_a = (it + DA - 1) * KG + group, st_b = (it + DB - 1) * KG + group;
+    const typename TA::Stage ga = ta.at(st_a);
+    const typename TB::Stage gb = tb.at(st_b);
+    const char* const sa = ring_a + now_a * TA::BYTES;
+    const char* const sb = ring_b + now_b * TB::BYTES;
+    i32x4 fa[MT][4], fb[4];
+    fp8_load<0, 4>(sb, wn * NT * 32, fb);
 #pragma unroll
-    for (int i = 0; i < MT; ++i) {
-      const i32x8 f0 = fp8_frag(sa, i * 32, 0), f1 = fp8_frag(sa, i * 32, 1);
+    for (int i = 0; i < MT; ++i) fp8_load<0, 4>(sa, (wm * MT + i) * 32, fa[i]);
+    f32x16 z[2], zero;
 #pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        f32x16 z;
+    for (int r = 0; r < 16; ++r) zero[r] = 0.0f;
+    // tiles in the order (j, i), j the slow one; u: the tile whose products are taken while t is scaled
 #pragma unroll
-        for (int r = 0; r < 16; ++r) z[r] = 0.0f;
-        z = fp8_mfma<E5M2>(fb[j][0], f0, z);
-        z = fp8_mfma<E5M2>(fb[j][1], f1, z);
+    for (int u = 0; u <= TILES; ++u) {
+      const int t = u - 1, i = u % MT, j = u / MT;
+      constexpr int PER = (2 * PASSES + TILES - 1) / TILES;  // passes a tile, in the first half of the tiles
 #pragma unroll
-        for (int r = 0; r < 16; ++r) acc[i][j][r] = fmaf(z[r], s_now[i], acc[i][j][r]);
+      for (int h = 0; h < 2; ++h) {
+        if (u < TILES) {
+          z[u & 1] = fp8_half<E5M2, !OUT16>(fb, fa[i], h, h ? z[u & 1] : zero);
+          // the last use of this half of the column fragment: the next one's takes its registers
+          if (i == MT - 1 && j + 1 < NT) {
+            __builtin_amdgcn_sched_barrier(0);
+            if (h == 0) fp8_load<0, 2>(sb, (wn * NT + j + 1) * 32, fb);
+            else fp8_load<2, 4>(sb, (wn * NT + j + 1) * 32, fb);
+          }
+        }
+        if (t >= 0) {
+#pragma unroll
+          for (int r = 8 * h; r < 8 * h + 8; ++r) acc[t % MT][t / MT][r] = fmaf(z[t & 1][r], scale[t % MT], acc[t % MT][t / MT][r]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+#pragma unroll
+      for (int q = u * PER; q < (u + 1) * PER && q < PASSES; ++q) {
+        if (q < TB::LOADS) tb.pass(ring_b + next_b * TB::BYTES, gb, st_b, q);
+        else ta.pass(ring_a + next_a * TA::BYTES, ga, st_a, q - TB::LOADS);
       }
     }
+    now_a = now_a + 1 == DA ? 0 : now_a + 1;
+    next_a = next_a + 1 == DA ? 0 : next_a + 1;
+    now_b = now_b + 1 == DB ? 0 : now_b + 1;
+    next_b = next_b + 1 == DB ? 0 : next_b + 1;
+  }
+  drain_loads();
+  if constexpr (KG > 1) {
+    float* const sums = (float*)smem;
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        __syncthreads();
+        if (group > 0) {
+#pragma unroll
+          for (int g = 0; g < 4; ++g)
+            *(f32x4*)&sums[(((group - 1) * 4 + g) * NTH + tid) * 4] =
+                f32x4{acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
+        }
+        __syncthreads();
+        if (group == 0) {
+#pragma unroll
+          for (int o = 0; o < KG - 1; ++o)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+              const f32x4 v = *(const f32x4*)&sums[((o * 4 + g) * NTH + tid) * 4];
+#pragma unroll
+              for (int r = 0; r < 4; ++r) acc[i][j][4 * g + r] += v[r];
+            }
+        }
+      }
+    if (group > 0) return;
   }
 #pragma unroll
   for (int j = 0; j < NT; ++j) {
@@ -348,44 +423,77 @@ __global__ __launch_bounds__(WM * WN * 64) void fp8_tile_kernel(Fp8Args a) {
         const float v = acc[i][j][r] + add[r];
         acc[i][j][r] = a.relu && v < 0.0f ? 0.0f : v;
       }
-      store_tile<OUT16>(acc[i][j], m < p.hi && n < a.n ? (char*)((out_t*)a.y + m * a.ldy + n) : nullptr, a.n - n, a.wide);
+      store_tile<OUT16>(acc[i][j], m < p.hi && n < a.n ? (char*)((out_t*)a.y + m * a.ldy + n) : nullptr, a.n - n);
     }
   }
 }
 
-template <bool E5M2, bool VEC, bool OUT16>
-int launch_fp8(Fp8Args a, hipStream_t stream) {
-  constexpr int BM = 128, BN = 128;
+template <bool E5M2, int WM, int WN, int MT, int NT, int KG, int DB, bool VEC, bool OUT16>
+int launch_tiles(FewArgs a, hipStream_t stream) {
+  constexpr int BM = WM * MT * 32, BN = WN * NT * 32;
   a.ntiles = (a.n + BN - 1) / BN;
   const unsigned grid = place_grid(BM, a.groups, a.offsets != nullptr, a.rows, a.ntiles);
   if (!grid) return C2D_ERR_UNSUPPORTED;
-  hipLaunchKernelGGL((fp8_tile_kernel<E5M2, 2, 2, 2, 2, VEC, OUT16>), dim3(grid), dim3(256), 0, stream, a);
+  hipLaunchKernelGGL((fp8_tile_kernel<E5M2, WM, WN, MT, NT, KG, DB, VEC, OUT16>), dim3(grid), dim3(WM * WN * KG * 64), 0, stream, a);
   return c2d_launch_status();
+}
+
+// Which kernel: the one whose estimated time is least, t = rounds of resident workgroups * (us per block of k *
+// blocks + us per round), with the rates that each was measured at (us; a workgroup per CU, 128 rows of 4096 x 4096
+// and up):
+//                             a round   a block of k     measured, rows x n x k: this, and the next larger / smaller
+//   256 x 256 tiles             3.5       1.95           8192 x 8192 x 8192: 509, in 128 x 128 tiles 680
+//   128 x 128, two per CU       3.5       1.30  (0.75    1024 x 4096 x 4096:  27, in 256 x 256 tiles 53
+//                                          one per CU)    2000 x 2000 x 256:  7.4, in 64 x 64 tiles 15.7
+//   64 x 64, two K groups       3.5       0.28           256 x 4096 x 4096: 13.6, in 128 x 128 tiles 27.5
+//                                                        2000 x 416 x 1024:  6.2, in 128 x 128 tiles 10.2
+//   32 x 32 from registers      2.5       0.29           256 x 1024 x 1024:  4.9, in 64 x 64 tiles 6.0
+// Up to 16 rows a group, 16 x 16 tiles from registers: the weights' way is all there is (1 x 8192 x 4096: 8.1 us,
+// 64 x 64 tiles 12.4; 16 x 4096 x 4096: 7.7 against 12.5).  An fp32 result doubles the matrix instructions and the
+// registers of a block's products; it has no 256 x 256 tiles, whose registers it would spill, nor have
+// operands that pass through registers on their way to LDS.
+template <bool E5M2, bool VEC, bool OUT16>
+int launch_fp8(const FewArgs& a, hipStream_t stream) {
+  constexpr int KIND = OUT16 ? FP8 : FP8_WIDE;
+  const int groups = a.offsets ? min(a.groups, a.rows) : 1;
+  if ((long long)a.rows <= 16ll * groups) return launch_few<KIND, E5M2, 1, 1, 8, VEC, OUT16>(a, stream);
+  auto tiles = [&](int side) {  // (a group's last row tile is half full, on average)
+    const double rows = a.offsets ? (double)a.rows / side + 0.5 * groups : (double)((a.rows + side - 1) / side);
+    return rows * ((a.n + side - 1) / side);
+  };
+  auto rounds = [](double t, double slots) { return t <= slots ? 1.0 : t / slots; };
+  const double kb = a.kb, wide = OUT16 ? 1.0 : 1.5;
+  const double t128 = tiles(128);
+  const double us256 = rounds(tiles(256), 256) * (1.95 * kb + 3.5);
+  const double us128 = t128 <= 256 ? 0.75 * wide * kb + 3.5 : rounds(t128, 512) * (1.3 * wide * kb + 3.5);
+  const double us64 = rounds(tiles(64), 256) * (0.28 * wide * kb + 3.5);
+  const double us32 = rounds(tiles(32), 256) * 0.29 * kb + 2.5;
+  if (OUT16 && VEC && us256 <= us128 && us256 <= us64 && us256 <= us32)
+    return launch_tiles<E5M2, 4, 2, 2, 4, 1, 2, true, true>(a, stream);
+  if (us128 <= us64 && us128 <= us32) return launch_tiles<E5M2, 2, 2, 2, 2, 1, 2, VEC, OUT16>(a, stream);
+  if (us64 <= us32) return launch_tiles<E5M2, 2, 2, 1, 1, 2, 4, VEC, OUT16>(a, stream);
+  return launch_few<KIND, E5M2, 2, 2, 8, VEC, OUT16>(a, stream);
 }
 
 }  // namespace
 
-extern "C" unsigned long long c2dp_fp8_matmul_workspace_bytes(int groups, int rows, int n, int k) {
-  (void)groups; (void)rows; (void)n; (void)k;
-  return 0;
-}
-
 extern "C" int c2dp_fp8_matmul(const void* a_, int a_type, long long lda, const float* a_scale, const void* b,
                                const float* b_scale, const int32_t* offsets, int groups, const float* bias, int relu,
                                void* y, int y_type, long long ldy, int rows, int n, int k, int clear_rest,
-                               void* workspace, unsigned long long workspace_bytes, void* stream) {
+                               void* stream) {
   C2D_CHECK_ARG(a_type == C2DP_E4M3 || a_type == C2DP_E5M2);
   C2D_CHECK_ARG(y_type == C2DP_F32 || y_type == C2DP_BF16);
   C2D_CHECK_ARG(groups > 0 && (offsets || groups == 1) && rows >= 0 && n >= 0 && k >= 0 && lda >= k && ldy >= n);
   if (rows == 0 || n == 0) return C2D_OK;
   C2D_CHECK_ARG(y && (k == 0 || (a_ && b && a_scale && b_scale)));
   if (lda > C2DP_MAX_PITCH || k > C2DP_MAX_PITCH) return C2D_ERR_UNSUPPORTED;
-  (void)workspace; (void)workspace_bytes;
-  Fp8Args a;
+  FewArgs a;
   a.a = (const char*)a_;
   a.lda = lda;
   a.a_scale = a_scale;
   a.b = (const char*)b;
+  a.ldb = k;
+  a.b_group = (long long)n * k;
   a.b_scale = b_scale;
   a.offsets = offsets;
   a.bias = bias;
@@ -397,7 +505,6 @@ extern "C" int c2dp_fp8_matmul(const void* a_, int a_type, long long lda, const 
   a.k = k;
   a.kb = (k + 127) / 128;
   a.nb = (n + 127) / 128;
-  a.wide = aligned16(y, ldy * (y_type == C2DP_BF16 ? 2 : 4));
   a.clear = clear_rest;
   a.relu = relu;
   const bool vec = aligned16(a_, lda) && aligned16(b, k);

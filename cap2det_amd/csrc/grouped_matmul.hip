@@ -3,6 +3,13 @@
 #include "products_common.h"
 
 using namespace c2d_pr;
+#ifndef XWM
+#define XWM 2
+#define XWN 2
+#define XMT 2
+#define XNT 2
+#define XD 2
+#endif
 
 namespace {
 
@@ -15,7 +22,7 @@ struct RowsArgs {             // forward and input gradient: one row of the resu
   char* y;
   long long ldy;              // elements
   int groups, rows, n, k;     // n: result columns, k: contraction
-  int ntiles, wide, clear;
+  int ntiles, clear;
 };
 
 struct WgradArgs {
@@ -24,12 +31,12 @@ struct WgradArgs {
   const int* offsets;
   float* dw;                  // [groups][n][k], or [splits][groups][n][k]
   int groups, rows, n, k;
-  int ntiles, ktiles, splits, wide, accumulate;
+  int ntiles, ktiles, splits, accumulate;
 };
 
-// Two buffers of a stage of A and B; while one is multiplied the other is loaded.  One barrier per
-// stage.  D[m][n], this wave's MT x NT tiles of 32 x 32.
-template <int ES, bool TRA, bool TRB, int WM, int WN, int MT, int NT, bool VEC>
+// A ring of D buffers, each a stage of A and B: while one is multiplied the next D - 1 are on their way.  One
+// barrier per stage.  D[m][n], this wave's MT x NT tiles of 32 x 32.
+template <int ES, bool TRA, bool TRB, int WM, int WN, int MT, int NT, int D, bool VEC>
 struct Core {
   static constexpr int BM = WM * MT * 32, BN = WN * NT * 32, NTH = WM * WN * 64;
   typedef Tile<ES, TRA, BM, NTH, VEC> TA;
@@ -63,29 +70,38 @@ struct Core {
       }
     }
   }
+  typedef typename std::conditional<ES == 2, bf16x8, f32x4>::type frag_t;
+
+  static __device__ __forceinline__ void load(const char* sa, const char* sb, int wm, int wn, int s, frag_t (&fa)[MT], frag_t (&fb)[NT]) {
+#pragma unroll
+    for (int j = 0; j < NT; ++j) fb[j] = frag<TRB, BN>(sb, (wn * NT + j) * 32, s);
+#pragma unroll
+    for (int i = 0; i < MT; ++i) fa[i] = frag<TRA, BM>(sa, (wm * MT + i) * 32, s);
+  }
 
   static __device__ __forceinline__ void stage(const char* sa, const char* sb, int wm, int wn, f32x16 (&acc)[MT][NT]) {
+    frag_t fa[2][MT], fb[2][NT];
+    load(sa, sb, wm, wn, 0, fa[0], fb[0]);
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
-      decltype(frag<TRA, BM>(sa, 0, 0)) fa[MT];
-      decltype(frag<TRB, BN>(sb, 0, 0)) fb[NT];
-#pragma unroll
-      for (int j = 0; j < NT; ++j) fb[j] = frag<TRB, BN>(sb, (wn * NT + j) * 32, s);
-#pragma unroll
-      for (int i = 0; i < MT; ++i) fa[i] = frag<TRA, BM>(sa, (wm * MT + i) * 32, s);
+      if (s < 3) load(sa, sb, wm, wn, s + 1, fa[(s + 1) & 1], fb[(s + 1) & 1]);
+      __builtin_amdgcn_sched_barrier(0);
       if constexpr (ES == 2) {
 #pragma unroll
         for (int i = 0; i < MT; ++i)
 #pragma unroll
-          for (int j = 0; j < NT; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fb[j], fa[i], acc[i][j], 0, 0, 0);
+          for (int j = 0; j < NT; ++j)
+            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fb[s & 1][j], fa[s & 1][i], acc[i][j], 0, 0, 0);
       } else {
 #pragma unroll
         for (int q = 0; q < 4; ++q)
 #pragma unroll
           for (int i = 0; i < MT; ++i)
 #pragma unroll
-            for (int j = 0; j < NT; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(fb[j][q], fa[i][q], acc[i][j], 0, 0, 0);
+            for (int j = 0; j < NT; ++j)
+              acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(fb[s & 1][j][q], fa[s & 1][i][q], acc[i][j], 0, 0, 0);
       }
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
 
@@ -96,27 +112,32 @@ struct Core {
       for (int j = 0; j < NT; ++j)
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
-    if (stages <= 0) return;
-    ta.issue(smem, first);
-    tb.issue(smem + TA::BYTES, first);
-    for (int it = 0; it < stages; ++it) {
-      char* const now = smem + (it & 1) * STAGE;
-      char* const next = smem + (~it & 1) * STAGE;
-      stage_barrier();
-      if (it + 1 < stages) {
-        ta.issue(next, first + it + 1);
-        tb.issue(next + TA::BYTES, first + it + 1);
+#pragma unroll
+    for (int d = 0; d < D - 1; ++d)
+      if (d < stages) {
+        ta.issue(smem + d * STAGE, first + d);
+        tb.issue(smem + d * STAGE + TA::BYTES, first + d);
       }
-      stage(now, now + TA::BYTES, wm, wn, acc);
+    int now = 0, next = D - 1;
+    for (int it = 0; it < stages; ++it) {
+      if (it + D - 1 <= stages) stage_barrier<VEC, (D - 2) * (TA::LOADS + TB::LOADS)>();
+      else stage_barrier<VEC, 0>();
+      if (it + D - 1 < stages) {
+        ta.issue(smem + next * STAGE, first + it + D - 1);
+        tb.issue(smem + next * STAGE + TA::BYTES, first + it + D - 1);
+      }
+      stage(smem + now * STAGE, smem + now * STAGE + TA::BYTES, wm, wn, acc);
+      now = now + 1 == D ? 0 : now + 1;
+      next = next + 1 == D ? 0 : next + 1;
     }
   }
 };
 
 // y = x . w^T (TRB false: w [n][k], the contraction along its rows) or dx = dy . w (TRB: across them).
-template <int ES, bool TRB, int WM, int WN, int MT, int NT, bool VEC, bool OUT16>
-__global__ __launch_bounds__(WM * WN * 64) void grouped_rows_kernel(RowsArgs a) {
-  typedef Core<ES, false, TRB, WM, WN, MT, NT, VEC> C;
-  __shared__ __attribute__((aligned(1024))) char smem[2 * C::STAGE];
+template <int ES, bool TRB, int WM, int WN, int MT, int NT, int D, bool VEC, bool OUT16>
+__global__ __launch_bounds__(WM * WN * 64, 2) void grouped_rows_kernel(RowsArgs a) {
+  typedef Core<ES, false, TRB, WM, WN, MT, NT, D, VEC> C;
+  __shared__ __attribute__((aligned(1024))) char smem[D * C::STAGE];
   typedef typename std::conditional<OUT16, __bf16, float>::type out_t;
   const Place p = place_tile<C::BM>(a.offsets, a.groups, a.rows, a.ntiles, blockIdx.x, gridDim.x);
   if (!p.live) {
@@ -138,16 +159,16 @@ __global__ __launch_bounds__(WM * WN * 64) void grouped_rows_kernel(RowsArgs a) 
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
       const int n = n0 + (wn * NT + j) * 32;
-      store_tile<OUT16>(acc[i][j], m < p.hi && n < a.n ? (char*)((out_t*)a.y + m * a.ldy + n) : nullptr, a.n - n, a.wide);
+      store_tile<OUT16>(acc[i][j], m < p.hi && n < a.n ? (char*)((out_t*)a.y + m * a.ldy + n) : nullptr, a.n - n);
     }
   }
 }
 
 // dw_e = dy_e^T . x_e.  Workgroup: group, tile of dw, and a share of the group's rows (whole stages).
-template <int ES, int WM, int WN, int MT, int NT, bool VEC>
-__global__ __launch_bounds__(WM * WN * 64) void grouped_wgrad_kernel(WgradArgs a) {
-  typedef Core<ES, true, true, WM, WN, MT, NT, VEC> C;
-  __shared__ __attribute__((aligned(1024))) char smem[2 * C::STAGE];
+template <int ES, int WM, int WN, int MT, int NT, int D, bool VEC>
+__global__ __launch_bounds__(WM * WN * 64, 2) void grouped_wgrad_kernel(WgradArgs a) {
+  typedef Core<ES, true, true, WM, WN, MT, NT, D, VEC> C;
+  __shared__ __attribute__((aligned(1024))) char smem[D * C::STAGE];
   const int tiles = a.ntiles * a.ktiles;
   const int e = blockIdx.x / (tiles * a.splits), at = blockIdx.x % (tiles * a.splits);
   const int split = at / tiles, nt = at % tiles / a.ktiles, kt = at % a.ktiles;
@@ -178,7 +199,7 @@ __global__ __launch_bounds__(WM * WN * 64) void grouped_wgrad_kernel(WgradArgs a
           if (k + c < a.k) acc[i][j][r] += row[c];
         }
       }
-      store_tile<false>(acc[i][j], (char*)row, a.k - k, a.wide);
+      store_tile<false>(acc[i][j], (char*)row, a.k - k);
     }
   }
 }
@@ -187,11 +208,12 @@ bool fits(long long pitch_bytes) { return pitch_bytes > 0 && pitch_bytes <= C2DP
 
 template <int ES, bool TRB, bool VEC, bool OUT16>
 int launch_rows(RowsArgs a, hipStream_t stream) {
-  constexpr int BM = 128, BN = 128;
+  constexpr int WM = XWM, WN = XWN, MT = XMT, NT = XNT, D = XD;
+  constexpr int BM = WM * MT * 32, BN = WN * NT * 32;
   a.ntiles = (a.n + BN - 1) / BN;
   const unsigned grid = place_grid(BM, a.groups, true, a.rows, a.ntiles);
   if (!grid) return C2D_ERR_UNSUPPORTED;
-  hipLaunchKernelGGL((grouped_rows_kernel<ES, TRB, 2, 2, 2, 2, VEC, OUT16>), dim3(grid), dim3(256), 0, stream, a);
+  hipLaunchKernelGGL((grouped_rows_kernel<ES, TRB, WM, WN, MT, NT, D, VEC, OUT16>), dim3(grid), dim3(WM * WN * 64), 0, stream, a);
   return c2d_launch_status();
 }
 
@@ -220,7 +242,6 @@ int rows_product(const void* x, int x_type, long long ldx, const void* w, const 
   a.rows = rows;
   a.n = n;
   a.k = contraction;
-  a.wide = aligned16(y, ldy * ys);
   a.clear = clear;
   const hipStream_t s = (hipStream_t)stream;
   // (16-byte loads: the contraction's last chunk is whole; across it, a row of w is whole chunks)
@@ -254,13 +275,14 @@ extern "C" unsigned long long c2dp_grouped_matmul_wgrad_workspace_bytes(int grou
 namespace {
 template <int ES, bool VEC>
 int launch_wgrad(WgradArgs a, hipStream_t stream) {
-  constexpr int BM = 128, BN = 128;
+  constexpr int WM = XWM, WN = XWN, MT = XMT, NT = XNT, D = XD;
+  constexpr int BM = WM * MT * 32, BN = WN * NT * 32;
   a.ntiles = (a.n + BM - 1) / BM;
   a.ktiles = (a.k + BN - 1) / BN;
   a.splits = 1;
   const long long grid = (long long)a.groups * a.ntiles * a.ktiles * a.splits;
   if (grid >= (1ll << 30)) return C2D_ERR_UNSUPPORTED;
-  hipLaunchKernelGGL((grouped_wgrad_kernel<ES, 2, 2, 2, 2, VEC>), dim3((unsigned)grid), dim3(256), 0, stream, a);
+  hipLaunchKernelGGL((grouped_wgrad_kernel<ES, WM, WN, MT, NT, D, VEC>), dim3((unsigned)grid), dim3(WM * WN * 64), 0, stream, a);
   return c2d_launch_status();
 }
 }  // namespace
@@ -287,7 +309,6 @@ extern "C" int c2dp_grouped_matmul_wgrad(const void* x, int x_type, long long ld
   a.rows = rows;
   a.n = n;
   a.k = k;
-  a.wide = aligned16(dw, (long long)k * 4);
   a.accumulate = accumulate;
   const bool vec = aligned16(x, a.ldx) && aligned16(dy, a.lddy) && n * es % 16 == 0 && k * es % 16 == 0;
   const hipStream_t s = (hipStream_t)stream;

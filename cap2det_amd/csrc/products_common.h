@@ -189,7 +189,7 @@ __device__ __forceinline__ void clear_rest(const Place& p, T* y, long long ldy, 
 //
 // VEC: loads go to LDS directly (buffer_load ... lds, 16 bytes a lane), and lie outside their buffer, which
 // returns zeros, behind the operand's last row and behind the contraction's end.  Not VEC (a pitch, a
-// pointer or a length that 16-byte loads do not fit): element loads with their own bounds.
+// pointer or a length that 16-byte loads to LDS do not fit): loads to registers, with their own bounds.
 template <int ES, bool TR, int R, int NTH, bool VEC>
 struct Tile {
   static constexpr int BYTES = R * 128;
@@ -204,72 +204,85 @@ struct Tile {
   const char* base;
   long long ld;          // bytes
   int across, len;       // rows (TR: columns) from base that exist; contraction elements
-  int row, chunk;        // this thread's staged row and source chunk of the first pass
-  unsigned off[LOADS];
-  __amdgpu_buffer_rsrc_t rs;
+  int tid, row, chunk;   // thread among the NTH, its staged row and source chunk of the first pass
+  unsigned off;          // its offset; pass i lies i * RPP rows behind it
 
-  __device__ __forceinline__ void begin(const void* p, long long ld_bytes, int across_, int len_) {
+  __device__ __forceinline__ void begin(const void* p, long long ld_bytes, int across_, int len_, int tid_ = threadIdx.x) {
+    tid = tid_;
     base = (const char*)p;
     ld = ld_bytes;
     across = min(across_, R);
     len = len_;
-    row = threadIdx.x / CPR;
-    const int pos = threadIdx.x % CPR;
+    row = tid / CPR;
+    const int pos = tid % CPR;
     chunk = !TR ? pos ^ ((row >> 1) & 7) : ES == 2 ? pos ^ ((row & 3) << 2) : pos;
-    if (VEC) {
-#pragma unroll
-      for (int i = 0; i < LOADS; ++i) off[i] = (unsigned)((row + i * RPP) * (int)ld + chunk * 16);
-      if (!TR) rs = buffer_of(base, across > 0 ? (long long)(across - 1) * ld + (long long)len * ES : 0);
-    }
+    off = (unsigned)(row * (int)ld + chunk * 16);
   }
 
-  // stage `st` into LDS at `to`
-  __device__ __forceinline__ void issue(char* to, int st) {
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // Where stage `st` begins, for the passes that follow: (TR) the buffer, else the lane's offset.
+  struct Stage { const char* base; long long bytes; unsigned off; int k0; };
+  __device__ __forceinline__ Stage at(int st) const {
+    Stage g;
+    if constexpr (TR) {
+      const long long k0 = (long long)st * KST, left = len - k0;
+      g.base = base + k0 * ld;
+      g.bytes = left > 0 && across > 0 ? (min(left, (long long)KST) - 1) * ld + (long long)across * ES : 0;
+      g.off = off;
+      g.k0 = 0;
+    } else {
+      g.base = base;
+      g.bytes = across > 0 ? (long long)(across - 1) * ld + (long long)len * ES : 0;
+      g.k0 = st * 128;
+      g.off = st * KST + chunk * EPC < len ? off : OUTSIDE;
+    }
+    return g;
+  }
+  // Pass i of stage `st` into LDS at `to`.  (The bound of a buffer holds for lane offset + scalar offset.)
+  __device__ __forceinline__ void pass(char* to, const Stage& g, int st, int i) const {
     if constexpr (VEC) {
-      if constexpr (TR) {
-        const long long k0 = (long long)st * KST;
-        const long long left = len - k0;
-        rs = buffer_of(base + k0 * ld, left > 0 && across > 0 ? (min(left, (long long)KST) - 1) * ld + (long long)across * ES : 0);
-#pragma unroll
-        for (int i = 0; i < LOADS; ++i)
-          __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void*)(to + i * NTH * 16 + wave * 1024), 16, (int)off[i], 0, 0, 0);
-      } else {
-        const int k0 = st * KST;
-        const bool in = k0 + chunk * EPC < len;
-#pragma unroll
-        for (int i = 0; i < LOADS; ++i)
-          __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void*)(to + i * NTH * 16 + wave * 1024), 16,
-                                                   (int)(in ? off[i] : OUTSIDE), k0 * ES, 0, 0);
-      }
+#ifdef __HIP_DEVICE_COMPILE__  // (the host pass refuses 16 bytes here, and with that drops some kernels' stubs)
+      const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(buffer_of(g.base, g.bytes), (lds_void*)(to + i * NTH * 16 + wave * 1024), 16, (int)g.off,
+                                               __builtin_amdgcn_readfirstlane(g.k0 + i * RPP * (int)ld), 0, 0);
+#endif
     } else {
       typedef typename std::conditional<ES == 1, unsigned char,
                                         typename std::conditional<ES == 2, unsigned short, unsigned>::type>::type elem_t;
       typedef elem_t chunk_t __attribute__((ext_vector_type(EPC)));
+      const int r = row + i * RPP;
+      const long long k = TR ? (long long)st * KST + r : (long long)st * KST + chunk * EPC;
+      const int a = TR ? chunk * EPC : r;
+      const char* const p = base + (TR ? k * ld + (long long)a * ES : a * ld + k * ES);
+      const long long left = k >= len || a >= across ? 0 : TR ? across - a : len - k;  // elements that exist
+      chunk_t v;
+      if (left >= EPC) {
+        __builtin_memcpy(&v, p, 16);
+      } else {
 #pragma unroll
-      for (int i = 0; i < LOADS; ++i) {
-        const int r = row + i * RPP;
-        chunk_t v;
-#pragma unroll
-        for (int j = 0; j < EPC; ++j) {
-          const long long k = TR ? (long long)st * KST + r : (long long)st * KST + chunk * EPC + j;
-          const int a = TR ? chunk * EPC + j : r;
-          v[j] = 0;
-          if (k < len && a < across)
-            v[j] = *(const elem_t*)(base + (TR ? k * ld + (long long)a * ES : a * ld + k * ES));
-        }
-        *(chunk_t*)(to + i * NTH * 16 + threadIdx.x * 16) = v;
+        for (int j = 0; j < EPC; ++j) v[j] = j < left ? ((const elem_t*)p)[j] : (elem_t)0;
       }
+      *(chunk_t*)(to + i * NTH * 16 + tid * 16) = v;
     }
+  }
+  __device__ __forceinline__ void issue(char* to, int st) const {
+    const Stage g = at(st);
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) pass(to, g, st, i);
   }
 };
 
-// All of this wave's loads to LDS have landed and its LDS reads are done; then the same of every wave.
+// All but the last `later` of this wave's loads to LDS have landed and its LDS reads and writes are done; then
+// the same of every wave.  (Not VEC: what a thread staged itself it has written by then.)
+template <bool VEC, int later>
 __device__ __forceinline__ void stage_barrier() {
-  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  static_assert(later <= 63, "a six-bit counter");
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(VEC ? later : 0) : "memory");
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
 }
+
+// No load to LDS is on its way any more: before the LDS is another workgroup's.
+__device__ __forceinline__ void drain_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
 // ---- result -----------------------------------------------------------------------------------------
 
@@ -280,12 +293,16 @@ __device__ __forceinline__ unsigned pack_bf16(float a, float b) {
   return __builtin_bit_cast(unsigned, v);
 }
 
+// 16 (8) bytes wherever they lie: global memory takes them at any address.
+template <class V>
+__device__ __forceinline__ void store_at(char* p, V v) { __builtin_memcpy(p, &v, sizeof(V)); }
+
 // A 32 x 32 result tile: lane l holds row m = l & 31, register r column 8 (r >> 2) + 4 (l >> 5) + (r & 3).
 // fp32: four 16-byte stores of 4 columns.  bf16: the halves of the wave exchange registers
 // (v_permlane32_swap) so that each holds 8 consecutive columns, two 16-byte stores.  `row`: this lane's row
 // of the result at the tile's first column, null if there is none; `cols`: columns that exist.
 template <bool BF16>
-__device__ __forceinline__ void store_tile(const f32x16& v, char* row, int cols, bool wide) {
+__device__ __forceinline__ void store_tile(const f32x16& v, char* row, int cols) {
   const int lh = (threadIdx.x >> 5) & 1;
   if constexpr (BF16) {
     unsigned w[8];
@@ -299,8 +316,8 @@ __device__ __forceinline__ void store_tile(const f32x16& v, char* row, int cols,
       const u32x4 o = {x[0], y[0], x[1], y[1]};  // columns 16 h + 8 lh .. + 7
       const int c = 16 * h + 8 * lh;
       if (row) {
-        if (wide && c + 8 <= cols) {
-          *(u32x4*)(row + c * 2) = o;
+        if (c + 8 <= cols) {
+          store_at(row + c * 2, o);
         } else {
 #pragma unroll
           for (int j = 0; j < 8; ++j)
@@ -313,8 +330,8 @@ __device__ __forceinline__ void store_tile(const f32x16& v, char* row, int cols,
     for (int g = 0; g < 4; ++g) {
       const int c = 8 * g + 4 * lh;
       if (row) {
-        if (wide && c + 4 <= cols) {
-          *(f32x4*)(row + c * 4) = f32x4{v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]};
+        if (c + 4 <= cols) {
+          store_at(row + c * 4, f32x4{v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]});
         } else {
 #pragma unroll
           for (int j = 0; j < 4; ++j)

@@ -4,6 +4,7 @@ PyTorch is plumbing only (allocation, streams); every arithmetic op on the hot p
 the hand-written HIP kernels behind these calls.  No fallback: a missing library raises.
 """
 import ctypes
+import functools
 
 import torch
 
@@ -846,77 +847,75 @@ def x9_planes(t):
 
 FP8_BLOCK = 128
 FP8_TYPES = (torch.float8_e4m3fn, torch.float8_e5m2)
+_WIDE_TYPES = (torch.float32, torch.bfloat16)
 _PRODUCT_TYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float8_e4m3fn: 2, torch.float8_e5m2: 3}
 
 
-def _need(ok, what):
-  if not ok:
-    raise ValueError(what)
+def _device():
+  """The current device's number (the private query that _stream uses costs a tenth of the public one)."""
+  return torch.cuda.current_device() if _cur_device is None else _cur_device()
 
 
-def _on_device(t, name):
-  _need(t.is_cuda, "%s: a device tensor is wanted, got one on %s" % (name, t.device))
-  _need(t.device.index == torch.cuda.current_device(),
-        "%s: on %s, but the current device is cuda:%d" % (name, t.device, torch.cuda.current_device()))
+def _names(types):
+  return ", ".join(str(t) for t in types)
 
 
-def _device_tensor(t, name, dtypes, dims):
-  _need(isinstance(t, torch.Tensor), "%s: a tensor is wanted, got %s" % (name, type(t).__name__))
-  _on_device(t, name)
-  _need(t.dtype in dtypes, "%s: one of %s is wanted, got %s" % (name, ", ".join(map(str, dtypes)), t.dtype))
-  _need(t.dim() in dims, "%s: %s dimensions are wanted, got shape %s" % (name, " or ".join(map(str, dims)),
-                                                                       tuple(t.shape)))
-  return t
+def _operand(t, name, types, dims, device):
+  """Refuses what is not a tensor of one of `types` with `dims` dimensions on the current device."""
+  if not isinstance(t, torch.Tensor):
+    raise ValueError("%s: a tensor is wanted, got %s" % (name, type(t).__name__))
+  if t.get_device() != device:
+    raise ValueError("%s: a tensor on the current device cuda:%d is wanted, got one on %s" % (name, device, t.device))
+  if t.dtype not in types:
+    raise ValueError("%s: one of %s is wanted, got %s" % (name, _names(types), t.dtype))
+  if t.dim() != dims:
+    raise ValueError("%s: %d dimensions are wanted, got shape %s" % (name, dims, tuple(t.shape)))
+
+
+def _whole(t, name, types, shape, device):
+  """The same, and a contiguous tensor of this shape."""
+  _operand(t, name, types, len(shape), device)
+  if t.shape != shape:
+    raise ValueError("%s: shape %s is wanted, got %s" % (name, tuple(shape), tuple(t.shape)))
+  if not t.is_contiguous():
+    raise ValueError("%s: has to be contiguous, got strides %s of shape %s" % (name, t.stride(), tuple(t.shape)))
 
 
 def _pitch(t, name):
   """Row pitch of a matrix in elements; columns have to be contiguous and rows apart."""
   rows, cols = t.shape
+  step, unit = t.stride()
+  if rows > 1 and unit == 1 and step >= cols:
+    return step
   if rows == 0 or cols == 0:
-    return max(cols, 1)
-  _need(cols == 1 or t.stride(1) == 1, "%s: columns have to be contiguous, got strides %s" % (name, t.stride()))
+    return cols
+  if cols > 1 and unit != 1:
+    raise ValueError("%s: columns have to be contiguous, got strides %s" % (name, (step, unit)))
   if rows == 1:
     return cols
-  _need(t.stride(0) >= cols, "%s: rows overlap, got strides %s of shape %s" % (name, t.stride(), tuple(t.shape)))
-  return t.stride(0)
-
-
-def _whole(t, name):
-  _need(t.is_contiguous(), "%s: has to be contiguous, got strides %s of shape %s" % (name, t.stride(), tuple(t.shape)))
-  return t
-
-
-def _group_offsets(offsets, groups):
-  _device_tensor(offsets, "offsets", (torch.int32,), (1,))
-  _need(offsets.numel() == groups + 1, "offsets: %d numbers are wanted for %d groups, got %d"
-        % (groups + 1, groups, offsets.numel()))
-  return _whole(offsets, "offsets")
-
-
-def _result(out, shape, dtypes, dtype, device, *inputs):
-  """(result tensor, whether rows in no group are to be cleared)."""
-  if out is None:
-    return torch.empty(shape, dtype=dtype, device=device), True
-  _device_tensor(out, "out", dtypes, (len(shape),))
-  _need(tuple(out.shape) == tuple(shape), "out: shape %s is wanted, got %s" % (tuple(shape), tuple(out.shape)))
-  lo, hi = _extent(out)
-  for t in inputs:
-    a, b = _extent(t)
-    _need(hi <= a or b <= lo, "out: shares memory with an operand")
-  return out, False
+  if step < cols:
+    raise ValueError("%s: rows overlap, got strides %s of shape %s" % (name, (step, unit), (rows, cols)))
+  return step
 
 
 def _extent(t):
   """First and last + 1 byte that a tensor reaches."""
-  if t is None or t.numel() == 0:
+  if t.numel() == 0:
     return 0, 0
   last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
   return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
 
 
-def _workspace(nbytes, device):
-  ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
-  return ws, (None if ws is None else ws.data_ptr()), nbytes
+def _given_result(out, shape, types, device, operands):
+  _operand(out, "out", types, len(shape), device)
+  if out.shape != shape:
+    raise ValueError("out: shape %s is wanted, got %s" % (tuple(shape), tuple(out.shape)))
+  lo, hi = _extent(out)
+  for t in operands:
+    if t is not None:
+      a, b = _extent(t)
+      if a < hi and lo < b:
+        raise ValueError("out: shares memory with an operand")
 
 
 def fp8_quantize(x, block_rows=1, dtype=torch.float8_e4m3fn):
@@ -927,46 +926,46 @@ def fp8_quantize(x, block_rows=1, dtype=torch.float8_e4m3fn):
   2^-126, F = 448 (float8_e4m3fn) or 57344 (float8_e5m2); q = x / scale in fp32, to the nearest, ties to
   even.  A NaN stays one and takes no part in the maximum, an infinity makes its block's values NaN.
   The blocks of a weight matrix w are square: q.t().contiguous() and scale.t().contiguous() are w.t()'s."""
-  _device_tensor(x, "x", (torch.float32, torch.bfloat16), (2, 3))
-  _need(dtype in FP8_TYPES, "dtype: one of %s is wanted, got %s" % (", ".join(map(str, FP8_TYPES)), dtype))
-  _need(block_rows in (1, FP8_BLOCK), "block_rows: 1 or %d, got %r" % (FP8_BLOCK, block_rows))
-  batch, (rows, cols) = (1 if x.dim() == 2 else x.shape[0]), x.shape[-2:]
-  lead = tuple(x.shape[:-2])
-  q = torch.empty(lead + (rows, cols), dtype=dtype, device=x.device)
-  scale = torch.empty(lead + (-(-rows // block_rows), -(-cols // FP8_BLOCK)), device=x.device)
-  if q.numel() == 0:
-    return q, scale
-  ld = _pitch(x if x.dim() == 2 else x[0], "x")
-  _lib.call("c2dp_fp8_quantize", x.data_ptr(), _PRODUCT_TYPE[x.dtype], ld, x.stride(0) if x.dim() == 3 else 0,
-            q.data_ptr(), _PRODUCT_TYPE[dtype], scale.data_ptr(), batch, rows, cols, block_rows, _stream())
+  _operand(x, "x", _WIDE_TYPES, 3 if isinstance(x, torch.Tensor) and x.dim() == 3 else 2, _device())
+  if dtype not in FP8_TYPES:
+    raise ValueError("dtype: one of %s is wanted, got %s" % (_names(FP8_TYPES), dtype))
+  if block_rows != 1 and block_rows != FP8_BLOCK:
+    raise ValueError("block_rows: 1 or %d, got %r" % (FP8_BLOCK, block_rows))
+  shape = x.shape
+  rows, cols = shape[-2], shape[-1]
+  grid = (-(-rows // block_rows), -(-cols // FP8_BLOCK))
+  if len(shape) == 2:
+    batch, step, ld = 1, 0, _pitch(x, "x")
+  else:
+    batch, step = shape[0], x.stride(0)
+    ld = _pitch(x[0], "x") if batch else cols
+    grid = (batch,) + grid
+  q = torch.empty(shape, dtype=dtype, device=x.device)
+  scale = torch.empty(grid, dtype=torch.float32, device=x.device)
+  if batch and rows and cols:
+    _lib.call("c2dp_fp8_quantize", x.data_ptr(), _PRODUCT_TYPE[x.dtype], ld, step, q.data_ptr(), _PRODUCT_TYPE[dtype],
+              scale.data_ptr(), batch, rows, cols, block_rows, _stream())
   return q, scale
 
 
-def _fp8_product(a, a_scale, b, b_scale, offsets, out, out_dtype, bias, relu):
-  groups, n, k = b.shape
+def _fp8_product(a, a_scale, b, b_scale, offsets, groups, n, k, out, out_dtype, bias, relu, device):
   rows = a.shape[0]
-  _need(a.shape[1] == k, "a: %d columns are wanted, got shape %s" % (k, tuple(a.shape)))
-  kb, nb = -(-k // FP8_BLOCK), -(-n // FP8_BLOCK)
-  _need(tuple(a_scale.shape) == (rows, kb), "a_scale: shape %s is wanted, got %s" % ((rows, kb), tuple(a_scale.shape)))
-  _need(b_scale.numel() == groups * nb * kb and tuple(b_scale.shape[-2:]) == (nb, kb),
-        "b_scale: shape %s is wanted, got %s" % ((groups, nb, kb), tuple(b_scale.shape)))
-  for t, name in ((a_scale, "a_scale"), (b, "b"), (b_scale, "b_scale")):
-    _whole(t, name)
-  if bias is not None:
-    _need(bias.numel() == groups * n and bias.shape[-1] == n, "bias: shape %s is wanted, got %s"
-          % ((groups, n), tuple(bias.shape)))
-    _whole(bias, "bias")
-  _need(out is not None or out_dtype in (torch.bfloat16, torch.float32),
-        "out_dtype: torch.bfloat16 or torch.float32, got %s" % (out_dtype,))
-  y, clear = _result(out, (rows, n), (torch.bfloat16, torch.float32), out_dtype, a.device, a, a_scale, b, b_scale,
-                     bias, offsets)
-  if y.numel() == 0:
-    return y
-  ws, ws_ptr, ws_bytes = _workspace(int(_lib.load().c2dp_fp8_matmul_workspace_bytes(groups, rows, n, k)), a.device)
-  _lib.call("c2dp_fp8_matmul", a.data_ptr(), _PRODUCT_TYPE[a.dtype], _pitch(a, "a"), a_scale.data_ptr(), b.data_ptr(),
-            b_scale.data_ptr(), None if offsets is None else offsets.data_ptr(), groups,
-            None if bias is None else bias.data_ptr(), int(bool(relu)), y.data_ptr(), _PRODUCT_TYPE[y.dtype],
-            _pitch(y, "out"), rows, n, k, int(clear), ws_ptr, ws_bytes, _stream())
+  if a.shape[1] != k:
+    raise ValueError("a: %d columns are wanted, got shape %s" % (k, tuple(a.shape)))
+  if out is None:
+    if out_dtype not in _WIDE_TYPES:
+      raise ValueError("out_dtype: one of %s is wanted, got %s" % (_names(_WIDE_TYPES), out_dtype))
+    y = torch.empty((rows, n), dtype=out_dtype, device=a.device)
+    ldy = n
+  else:
+    y = out
+    _given_result(y, (rows, n), _WIDE_TYPES, device, (a, a_scale, b, b_scale, bias, offsets))
+    ldy = _pitch(y, "out")
+  if rows and n:
+    _lib.call("c2dp_fp8_matmul", a.data_ptr(), _PRODUCT_TYPE[a.dtype], _pitch(a, "a"), a_scale.data_ptr(), b.data_ptr(),
+              b_scale.data_ptr(), None if offsets is None else offsets.data_ptr(), groups,
+              None if bias is None else bias.data_ptr(), 1 if relu else 0, y.data_ptr(), _PRODUCT_TYPE[y.dtype], ldy,
+              rows, n, k, 1 if out is None else 0, _stream())
   return y
 
 
@@ -975,86 +974,110 @@ def fp8_matmul(a, a_scale, b, b_scale, out=None, out_dtype=torch.bfloat16, bias=
   [rows, ceil(k / 128)] (fp8_quantize, block_rows 1; float8_e4m3fn, or float8_e5m2 as gradients use), b
   [n, k] float8_e4m3fn with b_scale [ceil(n / 128), ceil(k / 128)] (block_rows 128), bias [n] fp32 ->
   [rows, n] bf16 or fp32.  The input gradient is the same product on the transposed weight."""
-  _device_tensor(a, "a", FP8_TYPES, (2,))
-  _device_tensor(a_scale, "a_scale", (torch.float32,), (2,))
-  _device_tensor(b, "b", FP8_TYPES[:1], (2,))
-  _device_tensor(b_scale, "b_scale", (torch.float32,), (2,))
+  device = _device()
+  _operand(a, "a", FP8_TYPES, 2, device)
+  _operand(b, "b", FP8_TYPES[:1], 2, device)
+  n, k = b.shape
+  kb = -(-k // FP8_BLOCK)
+  _whole(b, "b", FP8_TYPES, (n, k), device)
+  _whole(a_scale, "a_scale", _WIDE_TYPES[:1], (a.shape[0], kb), device)
+  _whole(b_scale, "b_scale", _WIDE_TYPES[:1], (-(-n // FP8_BLOCK), kb), device)
   if bias is not None:
-    _device_tensor(bias, "bias", (torch.float32,), (1,))
-  return _fp8_product(a, a_scale, b.unsqueeze(0), b_scale, None, out, out_dtype, bias, relu)
+    _whole(bias, "bias", _WIDE_TYPES[:1], (n,), device)
+  return _fp8_product(a, a_scale, b, b_scale, None, 1, n, k, out, out_dtype, bias, relu, device)
 
 
 def grouped_matmul_fp8(a, a_scale, b, b_scale, offsets, out=None, out_dtype=torch.bfloat16, bias=None, relu=False):
   """fp8_matmul with one weight matrix per group of rows: b [groups, n, k], b_scale [groups, ceil(n / 128),
   ceil(k / 128)], bias [groups, n]."""
-  _device_tensor(a, "a", FP8_TYPES, (2,))
-  _device_tensor(a_scale, "a_scale", (torch.float32,), (2,))
-  _device_tensor(b, "b", FP8_TYPES[:1], (3,))
-  _device_tensor(b_scale, "b_scale", (torch.float32,), (3,))
+  device = _device()
+  _operand(a, "a", FP8_TYPES, 2, device)
+  _operand(b, "b", FP8_TYPES[:1], 3, device)
+  groups, n, k = b.shape
+  if groups == 0:
+    raise ValueError("b: at least one group is wanted, got shape %s" % (tuple(b.shape),))
+  kb = -(-k // FP8_BLOCK)
+  _whole(b, "b", FP8_TYPES, (groups, n, k), device)
+  _whole(a_scale, "a_scale", _WIDE_TYPES[:1], (a.shape[0], kb), device)
+  _whole(b_scale, "b_scale", _WIDE_TYPES[:1], (groups, -(-n // FP8_BLOCK), kb), device)
+  _whole(offsets, "offsets", (torch.int32,), (groups + 1,), device)
   if bias is not None:
-    _device_tensor(bias, "bias", (torch.float32,), (2,))
-  _need(b.shape[0] > 0, "b: at least one group is wanted, got shape %s" % (tuple(b.shape),))
-  return _fp8_product(a, a_scale, b, b_scale, _group_offsets(offsets, b.shape[0]), out, out_dtype, bias, relu)
+    _whole(bias, "bias", _WIDE_TYPES[:1], (groups, n), device)
+  return _fp8_product(a, a_scale, b, b_scale, offsets, groups, n, k, out, out_dtype, bias, relu, device)
 
 
-def _grouped_rows(name, x, w, offsets, out, out_dtype, n, k, result_cols, x_cols, x_name):
-  types = (torch.float32, torch.bfloat16)
-  _device_tensor(x, x_name, types, (2,))
-  _need(w.dtype == x.dtype, "w: %s as %s is wanted, got %s" % (x.dtype, x_name, w.dtype))
-  _need(x.shape[1] == x_cols, "%s: %d columns are wanted, got shape %s" % (x_name, x_cols, tuple(x.shape)))
-  _whole(w, "w")
-  _group_offsets(offsets, w.shape[0])
-  out_dtype = out_dtype or x.dtype
-  allowed = (torch.float32,) if x.dtype == torch.float32 else types
-  _need(out_dtype in allowed, "out_dtype: one of %s is wanted, got %s" % (", ".join(map(str, allowed)), out_dtype))
-  rows = x.shape[0]
-  y, clear = _result(out, (rows, result_cols), allowed, out_dtype, x.device, x, w, offsets)
-  if y.numel() == 0:
-    return y
-  _lib.call(name, x.data_ptr(), _PRODUCT_TYPE[x.dtype], _pitch(x, x_name), w.data_ptr(), offsets.data_ptr(), w.shape[0],
-            y.data_ptr(), _PRODUCT_TYPE[y.dtype], _pitch(y, "out"), rows, n, k, int(clear), _stream())
+def _grouped_rows(entry, x, name, w, offsets, out, out_dtype, dgrad):
+  device = _device()
+  _operand(x, name, _WIDE_TYPES, 2, device)
+  _operand(w, "w", (x.dtype,), 3, device)
+  groups, n, k = w.shape
+  if groups == 0:
+    raise ValueError("w: at least one group is wanted, got shape %s" % (tuple(w.shape),))
+  _whole(w, "w", (x.dtype,), (groups, n, k), device)
+  _whole(offsets, "offsets", (torch.int32,), (groups + 1,), device)
+  rows, cols, wide = x.shape[0], n if dgrad else k, k if dgrad else n
+  if x.shape[1] != cols:
+    raise ValueError("%s: %d columns are wanted, got shape %s" % (name, cols, tuple(x.shape)))
+  types = _WIDE_TYPES if x.dtype == torch.bfloat16 else _WIDE_TYPES[:1]
+  if out is None:
+    out_dtype = out_dtype or x.dtype
+    if out_dtype not in types:
+      raise ValueError("out_dtype: one of %s is wanted, got %s" % (_names(types), out_dtype))
+    y = torch.empty((rows, wide), dtype=out_dtype, device=x.device)
+    ldy = wide
+  else:
+    y = out
+    _given_result(y, (rows, wide), types, device, (x, w, offsets))
+    ldy = _pitch(y, "out")
+  if rows and wide:
+    _lib.call(entry, x.data_ptr(), _PRODUCT_TYPE[x.dtype], _pitch(x, name), w.data_ptr(), offsets.data_ptr(), groups,
+              y.data_ptr(), _PRODUCT_TYPE[y.dtype], ldy, rows, n, k, 1 if out is None else 0, _stream())
   return y
-
-
-def _group_weights(w):
-  _device_tensor(w, "w", (torch.float32, torch.bfloat16), (3,))
-  _need(w.shape[0] > 0, "w: at least one group is wanted, got shape %s" % (tuple(w.shape),))
-  return w.shape
 
 
 def grouped_matmul(x, w, offsets, out=None, out_dtype=None):
   """x_e . w_e^T for every group e of rows: x [rows, k], w [groups, n, k], both fp32 or both bf16 -> [rows, n] of
   x's type (bf16 operands: or fp32, by out_dtype or by `out`); fp32 sums."""
-  _, n, k = _group_weights(w)
-  return _grouped_rows("c2dp_grouped_matmul", x, w, offsets, out, out_dtype, n, k, n, k, "x")
+  return _grouped_rows("c2dp_grouped_matmul", x, "x", w, offsets, out, out_dtype, False)
 
 
 def grouped_matmul_dgrad(dy, w, offsets, out=None, out_dtype=None):
   """Input gradient of grouped_matmul: dy [rows, n], w [groups, n, k] -> dx [rows, k] = dy_e . w_e."""
-  _, n, k = _group_weights(w)
-  return _grouped_rows("c2dp_grouped_matmul_dgrad", dy, w, offsets, out, out_dtype, n, k, k, n, "dy")
+  return _grouped_rows("c2dp_grouped_matmul_dgrad", dy, "dy", w, offsets, out, out_dtype, True)
 
 
 def grouped_matmul_wgrad(x, dy, offsets, out=None, accumulate=False):
   """Weight gradient of grouped_matmul: x [rows, k], dy [rows, n] -> dw [groups, n, k] fp32, dw_e =
   dy_e^T . x_e, zero for an empty group; accumulate=True adds that to `out`.  The same call gives the same
   bits."""
-  types = (torch.float32, torch.bfloat16)
-  _device_tensor(x, "x", types, (2,))
-  _device_tensor(dy, "dy", (x.dtype,), (2,))
-  _need(dy.shape[0] == x.shape[0], "dy: %d rows are wanted, got shape %s" % (x.shape[0], tuple(dy.shape)))
-  _device_tensor(offsets, "offsets", (torch.int32,), (1,))
-  groups, rows, n, k = offsets.numel() - 1, x.shape[0], dy.shape[1], x.shape[1]
-  _need(groups > 0, "offsets: at least two numbers are wanted, got %d" % offsets.numel())
-  _group_offsets(offsets, groups)
-  _need(out is not None or not accumulate, "accumulate: there is no `out` to add to")
-  dw, _ = _result(out, (groups, n, k), (torch.float32,), torch.float32, x.device, x, dy, offsets)
-  _whole(dw, "out")
-  if dw.numel() == 0:
-    return dw
-  ws, ws_ptr, ws_bytes = _workspace(
-      int(_lib.load().c2dp_grouped_matmul_wgrad_workspace_bytes(groups, rows, n, k)), x.device)
-  _lib.call("c2dp_grouped_matmul_wgrad", x.data_ptr(), _PRODUCT_TYPE[x.dtype], _pitch(x, "x"), dy.data_ptr(),
-            _pitch(dy, "dy"), offsets.data_ptr(), groups, dw.data_ptr(), rows, n, k,
-            int(bool(accumulate)), ws_ptr, ws_bytes, _stream())
+  device = _device()
+  _operand(x, "x", _WIDE_TYPES, 2, device)
+  _operand(dy, "dy", (x.dtype,), 2, device)
+  _operand(offsets, "offsets", (torch.int32,), 1, device)
+  rows, k = x.shape
+  n, groups = dy.shape[1], offsets.numel() - 1
+  if dy.shape[0] != rows:
+    raise ValueError("dy: %d rows are wanted, got shape %s" % (rows, tuple(dy.shape)))
+  if groups < 1:
+    raise ValueError("offsets: at least two numbers are wanted, got %d" % offsets.numel())
+  _whole(offsets, "offsets", (torch.int32,), (groups + 1,), device)
+  if out is None:
+    if accumulate:
+      raise ValueError("accumulate: there is no `out` to add to")
+    dw = torch.empty((groups, n, k), dtype=torch.float32, device=x.device)
+  else:
+    dw = out
+    _whole(dw, "out", _WIDE_TYPES[:1], (groups, n, k), device)
+    _given_result(dw, (groups, n, k), _WIDE_TYPES[:1], device, (x, dy, offsets))
+  if groups and n and k:
+    nbytes = _wgrad_workspace_bytes(groups, rows, n, k)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
+    _lib.call("c2dp_grouped_matmul_wgrad", x.data_ptr(), _PRODUCT_TYPE[x.dtype], _pitch(x, "x"), dy.data_ptr(),
+              _pitch(dy, "dy"), offsets.data_ptr(), groups, dw.data_ptr(), rows, n, k, 1 if accumulate else 0,
+              None if ws is None else ws.data_ptr(), nbytes, _stream())
   return dw
+
+
+@functools.lru_cache(maxsize=1024)
+def _wgrad_workspace_bytes(groups, rows, n, k):
+  return int(_lib.load().c2dp_grouped_matmul_wgrad_workspace_bytes(groups, rows, n, k))

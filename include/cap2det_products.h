@@ -9,7 +9,7 @@
  *   - a type argument is one of the C2DP_* numbers below.
  *   - a pitch is at most C2DP_MAX_PITCH bytes, else C2D_ERR_UNSUPPORTED.  16-byte aligned base
  *     pointers, pitches and contraction lengths take the direct global -> LDS loads; any others are
- *     right too, through element loads, and slower.
+ *     right too, through registers, and slower.
  *   - sums are fp32.
  *
  * Groups.  `offsets` is a DEVICE array of groups + 1 int32 row numbers: group e owns the rows
@@ -58,14 +58,10 @@ int c2dp_fp8_quantize(const void* x, int x_type, long long ldx, long long x_batc
  *   b_scale [groups][ceil(n / 128)][ceil(k / 128)]
  *   offsets NULL with groups == 1: every row belongs to the one matrix
  *   bias    [groups][n] fp32 or NULL;  relu != 0 applies max(., 0)
- *   y       [rows][n]       C2DP_F32 or C2DP_BF16 (y_type), pitch ldy
- *   workspace: c2dp_fp8_matmul_workspace_bytes(...) bytes, 16-byte aligned (may be NULL when that is 0);
- *   its contents need not be set, and calls that may run at the same time need one each. */
-unsigned long long c2dp_fp8_matmul_workspace_bytes(int groups, int rows, int n, int k);
+ *   y       [rows][n]       C2DP_F32 or C2DP_BF16 (y_type), pitch ldy */
 int c2dp_fp8_matmul(const void* a, int a_type, long long lda, const float* a_scale, const void* b,
                     const float* b_scale, const int32_t* offsets, int groups, const float* bias, int relu,
-                    void* y, int y_type, long long ldy, int rows, int n, int k, int clear_rest,
-                    void* workspace, unsigned long long workspace_bytes, void* stream);
+                    void* y, int y_type, long long ldy, int rows, int n, int k, int clear_rest, void* stream);
 
 /* y[i][j] = sum_k x[i][k] * w[e][j][k], e the group of row i.  x and w are both C2DP_F32 or both
  * C2DP_BF16 (x_type); y_type is x_type, or C2DP_F32 for bf16 operands.
@@ -84,7 +80,8 @@ int c2dp_grouped_matmul_dgrad(const void* dy, int dy_type, long long lddy, const
  * is zero), or dw += that when accumulate is not 0.  dy and x share x_type.  The rows of a group may be
  * dealt to several workgroups; their sums are joined in a fixed order (no atomics).
  *   x [rows][k] pitch ldx;  dy [rows][n] pitch lddy;  dw [groups][n][k] contiguous
- *   workspace: c2dp_grouped_matmul_wgrad_workspace_bytes(...) bytes, as above */
+ *   workspace: c2dp_grouped_matmul_wgrad_workspace_bytes(...) bytes, 16-byte aligned (may be NULL when that is
+ *   0); its contents need not be set, and calls that may run at the same time need one each. */
 unsigned long long c2dp_grouped_matmul_wgrad_workspace_bytes(int groups, int rows, int n, int k);
 int c2dp_grouped_matmul_wgrad(const void* x, int x_type, long long ldx, const void* dy, long long lddy,
                               const int32_t* offsets, int groups, float* dw, int rows, int n, int k,
