@@ -264,23 +264,25 @@ __device__ __forceinline__ f32x16 fp8_half(const i32x4 (&b)[4], const i32x4 (&a)
 // joined through LDS, in the groups' order.  A stage of a small tile is a chain of waits (barrier, LDS read, two
 // matrix instructions, scaling) of 0.5 us whatever its size (64 x 64 tiles): where there is a workgroup per CU
 // or less, KG chains run side by side (256 x 4096 x 4096: 17.6 us, with two groups 13.6, with four 14.6).
-template <bool E5M2, int WM, int WN, int MT, int NT, int KG, int DB, bool VEC, bool OUT16>
-__global__ __launch_bounds__(WM * WN * KG * 64, 2) void fp8_tile_kernel(FewArgs a) {
-  constexpr int BM = WM * MT * 32, BN = WN * NT * 32, NTH = WM * WN * 64, DA = DB + 1, TILES = MT * NT;
+template <bool E5M2, int WM, int WN, int MT, int NT, int KG, int DB, bool VEC>
+struct Fp8Tiles {
+  static constexpr int BM = WM * MT * 32, BN = WN * NT * 32, NTH = WM * WN * 64, DA = DB + 1, TILES = MT * NT;
   typedef Tile<1, false, BM, NTH, VEC> TA;
   typedef Tile<1, false, BN, NTH, VEC> TB;
-  constexpr int PASSES = TA::LOADS + TB::LOADS;
-  constexpr int RING = DA * TA::BYTES + DB * TB::BYTES;
+  static constexpr int PASSES = TA::LOADS + TB::LOADS;
+  static constexpr int RING = DA * TA::BYTES + DB * TB::BYTES;
   static_assert(128 % (NT * 32) == 0, "a wave's columns share a block of b");
   static_assert(KG == 1 || (KG - 1) * NTH * 64 <= KG * RING, "the sums are joined a tile at a time in the ring's LDS");
-  __shared__ __attribute__((aligned(1024))) char smem[KG * RING];
+};
+
+// A row tile (`p`) of BM rows or less.
+template <bool E5M2, int WM, int WN, int MT, int NT, int KG, int DB, bool VEC, bool OUT16>
+__device__ __forceinline__ void fp8_tile(const FewArgs& a, const Place& p, char* smem, int group, int tid) {
+  typedef Fp8Tiles<E5M2, WM, WN, MT, NT, KG, DB, VEC> C;
+  constexpr int BN = C::BN, NTH = C::NTH, DA = C::DA, TILES = C::TILES, PASSES = C::PASSES, RING = C::RING;
+  typedef typename C::TA TA;
+  typedef typename C::TB TB;
   typedef typename std::conditional<OUT16, __bf16, float>::type out_t;
-  const Place p = place_tile<BM>(a.offsets, a.groups, a.rows, a.ntiles, blockIdx.x, gridDim.x);
-  if (!p.live) {
-    if (a.clear) clear_rest(p, (out_t*)a.y, a.ldy, a.rows, a.n, NTH * KG);
-    return;
-  }
-  const int group = KG == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / NTH), tid = threadIdx.x - group * NTH;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / WN, wn = wave % WN;
   const int lane = threadIdx.x & 63, li = lane & 31, lh = lane >> 5;
@@ -380,30 +382,7 @@ __global__ __launch_bounds__(WM * WN * KG * 64, 2) void fp8_tile_kernel(FewArgs 
   }
   drain_loads();
   if constexpr (KG > 1) {
-    float* const sums = (float*)smem;
-#pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        __syncthreads();
-        if (group > 0) {
-#pragma unroll
-          for (int g = 0; g < 4; ++g)
-            *(f32x4*)&sums[(((group - 1) * 4 + g) * NTH + tid) * 4] =
-                f32x4{acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
-        }
-        __syncthreads();
-        if (group == 0) {
-#pragma unroll
-          for (int o = 0; o < KG - 1; ++o)
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-              const f32x4 v = *(const f32x4*)&sums[((o * 4 + g) * NTH + tid) * 4];
-#pragma unroll
-              for (int r = 0; r < 4; ++r) acc[i][j][4 * g + r] += v[r];
-            }
-        }
-      }
+    join_groups<KG, NTH>((float*)smem, group, tid, acc);
     if (group > 0) return;
   }
 #pragma unroll
@@ -428,6 +407,27 @@ __global__ __launch_bounds__(WM * WN * KG * 64, 2) void fp8_tile_kernel(FewArgs 
   }
 }
 
+// A group's last tile is on average half full.  Half of it or less is multiplied as a tile of half the height.
+template <bool E5M2, int WM, int WN, int MT, int NT, int KG, int DB, bool VEC, bool OUT16>
+__global__ __launch_bounds__(WM * WN * KG * 64, 2) void fp8_tile_kernel(FewArgs a) {
+  typedef Fp8Tiles<E5M2, WM, WN, MT, NT, KG, DB, VEC> C;
+  __shared__ __attribute__((aligned(1024))) char smem[KG * C::RING];
+  typedef typename std::conditional<OUT16, __bf16, float>::type out_t;
+  const Place p = place_tile<C::BM>(a.offsets, a.groups, a.rows, a.ntiles, blockIdx.x, gridDim.x);
+  if (!p.live) {
+    if (a.clear) clear_rest(p, (out_t*)a.y, a.ldy, a.rows, a.n, C::NTH * KG);
+    return;
+  }
+  const int group = KG == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / C::NTH), tid = threadIdx.x - group * C::NTH;
+  if constexpr (MT > 1) {
+    if (p.hi - p.m0 <= C::BM / 2) {
+      fp8_tile<E5M2, WM, WN, MT / 2, NT, KG, DB, VEC, OUT16>(a, p, smem, group, tid);
+      return;
+    }
+  }
+  fp8_tile<E5M2, WM, WN, MT, NT, KG, DB, VEC, OUT16>(a, p, smem, group, tid);
+}
+
 template <bool E5M2, int WM, int WN, int MT, int NT, int KG, int DB, bool VEC, bool OUT16>
 int launch_tiles(FewArgs a, hipStream_t stream) {
   constexpr int BM = WM * MT * 32, BN = WN * NT * 32;
@@ -448,7 +448,7 @@ int launch_tiles(FewArgs a, hipStream_t stream) {
 //   64 x 64, two K groups       3.5       0.28           256 x 4096 x 4096: 13.6, in 128 x 128 tiles 27.5
 //                                                        2000 x 416 x 1024:  6.2, in 128 x 128 tiles 10.2
 //   32 x 32 from registers      2.5       0.29           256 x 1024 x 1024:  4.9, in 64 x 64 tiles 6.0
-// Up to 16 rows a group, 16 x 16 tiles from registers: the weights' way is all there is (1 x 8192 x 4096: 8.1 us,
+// Up to 16 rows a group, 16-row tiles from registers: the weights' way is all there is (1 x 8192 x 4096: 8.1 us,
 // 64 x 64 tiles 12.4; 16 x 4096 x 4096: 7.7 against 12.5).  An fp32 result doubles the matrix instructions and the
 // registers of a block's products; it has no 256 x 256 tiles, whose registers it would spill, nor have
 // operands that pass through registers on their way to LDS.
@@ -456,9 +456,9 @@ template <bool E5M2, bool VEC, bool OUT16>
 int launch_fp8(const FewArgs& a, hipStream_t stream) {
   constexpr int KIND = OUT16 ? FP8 : FP8_WIDE;
   const int groups = a.offsets ? min(a.groups, a.rows) : 1;
-  if ((long long)a.rows <= 16ll * groups) return launch_few<KIND, E5M2, 1, 1, 8, VEC, OUT16>(a, stream);
-  auto tiles = [&](int side) {  // (a group's last row tile is half full, on average)
-    const double rows = a.offsets ? (double)a.rows / side + 0.5 * groups : (double)((a.rows + side - 1) / side);
+  if ((long long)a.rows <= 16ll * groups) return launch_sixteen_rows<KIND, E5M2, VEC, OUT16>(a, stream);
+  auto tiles = [&](int side) {  // (a group's last row tile counts for what it costs, on average)
+    const double rows = a.offsets ? (double)a.rows / side + 0.4 * groups : (double)((a.rows + side - 1) / side);
     return rows * ((a.n + side - 1) / side);
   };
   auto rounds = [](double t, double slots) { return t <= slots ? 1.0 : t / slots; };

@@ -1,29 +1,10 @@
 // Matrix products grouped by expert: the rows of x sorted by group, one weight matrix per group, the groups'
 // lengths on the device.  Forward, input gradient and weight gradient, bf16 and fp32 operands, fp32 sums.
-#include "products_common.h"
+#include "products_few.h"
 
 using namespace c2d_pr;
-#ifndef XWM
-#define XWM 2
-#define XWN 2
-#define XMT 2
-#define XNT 2
-#define XD 2
-#endif
 
 namespace {
-
-struct RowsArgs {             // forward and input gradient: one row of the result per row of A
-  const char* a;
-  long long lda;              // bytes
-  const char* w;
-  long long ldw, w_group;     // bytes
-  const int* offsets;
-  char* y;
-  long long ldy;              // elements
-  int groups, rows, n, k;     // n: result columns, k: contraction
-  int ntiles, clear;
-};
 
 struct WgradArgs {
   const char *dy, *x;
@@ -34,18 +15,23 @@ struct WgradArgs {
   int ntiles, ktiles, splits, accumulate;
 };
 
-// A ring of D buffers, each a stage of A and B: while one is multiplied the next D - 1 are on their way.  One
-// barrier per stage.  D[m][n], this wave's MT x NT tiles of 32 x 32.
-template <int ES, bool TRA, bool TRB, int WM, int WN, int MT, int NT, int D, bool VEC>
+// The stages of B go round DB buffers, those of A round DB + 1: while a stage is multiplied, the next of B and
+// the next two of A are on their way (DB = 2; two of each and a half are what the LDS holds of 256 x 256 tiles, and
+// a load takes longer than a stage).  One barrier per stage; the loads are issued between the matrix instructions of
+// its first half, since a burst of them behind the barrier holds up every wave of the workgroup.
+// KG > 1: KG groups of WM x WN waves share the tile, group g taking the stages g, g + KG, ..
+template <int ES, bool TRA, bool TRB, int WM, int WN, int MT, int NT, int KG, int DB, bool VEC>
 struct Core {
-  static constexpr int BM = WM * MT * 32, BN = WN * NT * 32, NTH = WM * WN * 64;
-  typedef Tile<ES, TRA, BM, NTH, VEC> TA;
-  typedef Tile<ES, TRB, BN, NTH, VEC> TB;
-  static constexpr int STAGE = TA::BYTES + TB::BYTES;
+  static constexpr int BM = WM * MT * 32, BN = WN * NT * 32, NTH = WM * WN * 64, DA = DB + 1;
+  typedef Tile<ES, TRA, BM, NTH, VEC, TRA || TRB> TA;
+  typedef Tile<ES, TRB, BN, NTH, VEC, TRA || TRB> TB;
+  static constexpr int RING = DA * TA::BYTES + DB * TB::BYTES;
+  static constexpr int PASSES = TA::LOADS + TB::LOADS;
   static constexpr int KST = TA::KST;
+  static_assert(KG == 1 || (KG - 1) * NTH * 64 <= KG * RING, "the sums are joined a tile at a time in the ring's LDS");
 
   // fragment of 32 rows (TR: columns) from `r0`, k-step s, for a lane
-  template <bool TR, int R>
+  template <class T, bool TR, int R>
   static __device__ __forceinline__ auto frag(const char* t, int r0, int s) {
     const int lane = threadIdx.x & 63, li = lane & 31, lh = lane >> 5;
     if constexpr (ES == 2) {
@@ -54,7 +40,7 @@ struct Core {
       } else {
         // rows 16 s + 8 lh + (0..3, 4..7): the transposed read hands lane l column l & 31 of them
         const int tq = (lane & 15) >> 2, tp = lane & 3, tg = (lane >> 4) & 1;
-        const char* p = t + (16 * s + 8 * lh + tq) * (R * 2) + (((r0 >> 5) ^ tq) << 6) + 32 * tg + 8 * tp;
+        const char* p = t + (16 * s + 8 * lh + tq) * (R * 2) + (((r0 >> 5) ^ (T::swizzle(tq) >> 2)) << 6) + 32 * tg + 8 * tp;
         const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p);
         const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + 4 * R * 2));
         return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
@@ -74,85 +60,96 @@ struct Core {
 
   static __device__ __forceinline__ void load(const char* sa, const char* sb, int wm, int wn, int s, frag_t (&fa)[MT], frag_t (&fb)[NT]) {
 #pragma unroll
-    for (int j = 0; j < NT; ++j) fb[j] = frag<TRB, BN>(sb, (wn * NT + j) * 32, s);
+    for (int j = 0; j < NT; ++j) fb[j] = frag<TB, TRB, BN>(sb, (wn * NT + j) * 32, s);
 #pragma unroll
-    for (int i = 0; i < MT; ++i) fa[i] = frag<TRA, BM>(sa, (wm * MT + i) * 32, s);
+    for (int i = 0; i < MT; ++i) fa[i] = frag<TA, TRA, BM>(sa, (wm * MT + i) * 32, s);
   }
 
-  static __device__ __forceinline__ void stage(const char* sa, const char* sb, int wm, int wn, f32x16 (&acc)[MT][NT]) {
-    frag_t fa[2][MT], fb[2][NT];
-    load(sa, sb, wm, wn, 0, fa[0], fb[0]);
-#pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      if (s < 3) load(sa, sb, wm, wn, s + 1, fa[(s + 1) & 1], fb[(s + 1) & 1]);
-      __builtin_amdgcn_sched_barrier(0);
-      if constexpr (ES == 2) {
-#pragma unroll
-        for (int i = 0; i < MT; ++i)
-#pragma unroll
-          for (int j = 0; j < NT; ++j)
-            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fb[s & 1][j], fa[s & 1][i], acc[i][j], 0, 0, 0);
-      } else {
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-#pragma unroll
-          for (int i = 0; i < MT; ++i)
-#pragma unroll
-            for (int j = 0; j < NT; ++j)
-              acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(fb[s & 1][j][q], fa[s & 1][i][q], acc[i][j], 0, 0, 0);
-      }
-      __builtin_amdgcn_sched_barrier(0);
-    }
-  }
-
-  static __device__ __forceinline__ void run(TA& ta, TB& tb, int first, int stages, char* smem, int wm, int wn, f32x16 (&acc)[MT][NT]) {
+  // Stages first .. first + stages - 1.
+  static __device__ __forceinline__ void run(const TA& ta, const TB& tb, int first, int stages, char* smem, int group, int wm,
+                                             int wn, f32x16 (&acc)[MT][NT]) {
 #pragma unroll
     for (int i = 0; i < MT; ++i)
 #pragma unroll
       for (int j = 0; j < NT; ++j)
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
+    if (stages <= 0) return;
+    char* const ring_a = smem + group * RING;
+    char* const ring_b = ring_a + DA * TA::BYTES;
+    const int rounds = (stages + KG - 1) / KG;
+    // (a stage behind the last reads zeros: the operands end there)
+    ta.issue(ring_a, first + group);
 #pragma unroll
-    for (int d = 0; d < D - 1; ++d)
-      if (d < stages) {
-        ta.issue(smem + d * STAGE, first + d);
-        tb.issue(smem + d * STAGE + TA::BYTES, first + d);
-      }
-    int now = 0, next = D - 1;
-    for (int it = 0; it < stages; ++it) {
-      if (it + D - 1 <= stages) stage_barrier<VEC, (D - 2) * (TA::LOADS + TB::LOADS)>();
-      else stage_barrier<VEC, 0>();
-      if (it + D - 1 < stages) {
-        ta.issue(smem + next * STAGE, first + it + D - 1);
-        tb.issue(smem + next * STAGE + TA::BYTES, first + it + D - 1);
-      }
-      stage(smem + now * STAGE, smem + now * STAGE + TA::BYTES, wm, wn, acc);
-      now = now + 1 == D ? 0 : now + 1;
-      next = next + 1 == D ? 0 : next + 1;
+    for (int d = 0; d < DB - 1; ++d) {
+      tb.issue(ring_b + d * TB::BYTES, first + d * KG + group);
+      ta.issue(ring_a + (d + 1) * TA::BYTES, first + (d + 1) * KG + group);
     }
+    int now_a = 0, now_b = 0, next_a = DA - 1, next_b = DB - 1;
+    for (int it = 0; it < rounds; ++it) {
+      // (behind this stage's B have been issued: A of the next, and DB - 2 whole stages)
+      stage_barrier<VEC, TA::LOADS + (DB - 2) * PASSES>();
+      const int st_a = first + (it + DA - 1) * KG + group, st_b = first + (it + DB - 1) * KG + group;
+      const typename TA::Stage ga = ta.at(st_a);
+      const typename TB::Stage gb = tb.at(st_b);
+      const char* const sa = ring_a + now_a * TA::BYTES;
+      const char* const sb = ring_b + now_b * TB::BYTES;
+      auto pass = [&](int q) {
+        if (q < TB::LOADS) tb.pass(ring_b + next_b * TB::BYTES, gb, st_b, q);
+        else ta.pass(ring_a + next_a * TA::BYTES, ga, st_a, q - TB::LOADS);
+      };
+      constexpr int QS = ES == 2 ? 1 : 4, SLOTS = 4 * QS * MT * NT;  // matrix instructions of a stage
+      constexpr int PER = (2 * PASSES + SLOTS - 1) / SLOTS, EVERY = PER > 1 ? 1 : SLOTS / (2 * PASSES);
+      frag_t fa[2][MT], fb[2][NT];
+      load(sa, sb, wm, wn, 0, fa[0], fb[0]);
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        if (s < 3) load(sa, sb, wm, wn, s + 1, fa[(s + 1) & 1], fb[(s + 1) & 1]);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int q = 0; q < QS; ++q)
+#pragma unroll
+          for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+              if constexpr (ES == 2)
+                acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fb[s & 1][j], fa[s & 1][i], acc[i][j], 0, 0, 0);
+              else
+                acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(fb[s & 1][j][q], fa[s & 1][i][q], acc[i][j], 0, 0, 0);
+              const int slot = ((s * QS + q) * MT + i) * NT + j;
+              if (slot % EVERY == 0) {
+#pragma unroll
+                for (int u = slot / EVERY * PER; u < (slot / EVERY + 1) * PER && u < PASSES; ++u) pass(u);
+                if (slot / EVERY * PER < PASSES) __builtin_amdgcn_sched_barrier(0);
+              }
+            }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      now_a = now_a + 1 == DA ? 0 : now_a + 1;
+      next_a = next_a + 1 == DA ? 0 : next_a + 1;
+      now_b = now_b + 1 == DB ? 0 : now_b + 1;
+      next_b = next_b + 1 == DB ? 0 : next_b + 1;
+    }
+    drain_loads();
+    if constexpr (KG > 1) join_groups<KG, NTH>((float*)smem, group, threadIdx.x - group * NTH, acc);
   }
 };
 
 // y = x . w^T (TRB false: w [n][k], the contraction along its rows) or dx = dy . w (TRB: across them).
-template <int ES, bool TRB, int WM, int WN, int MT, int NT, int D, bool VEC, bool OUT16>
-__global__ __launch_bounds__(WM * WN * 64, 2) void grouped_rows_kernel(RowsArgs a) {
-  typedef Core<ES, false, TRB, WM, WN, MT, NT, D, VEC> C;
-  __shared__ __attribute__((aligned(1024))) char smem[D * C::STAGE];
+// A row tile (`p`) of C's height or less.
+template <class C, bool TRB, int ES, int WN, int MT, int NT, bool OUT16>
+__device__ __forceinline__ void rows_tile(const FewArgs& a, const Place& p, char* smem, int group, int tid) {
   typedef typename std::conditional<OUT16, __bf16, float>::type out_t;
-  const Place p = place_tile<C::BM>(a.offsets, a.groups, a.rows, a.ntiles, blockIdx.x, gridDim.x);
-  if (!p.live) {
-    if (a.clear) clear_rest(p, (out_t*)a.y, a.ldy, a.rows, a.n, C::NTH);
-    return;
-  }
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / WN, wn = wave % WN;
   const int n0 = p.nt * C::BN;
   typename C::TA ta;
   typename C::TB tb;
-  ta.begin(a.a + (long long)p.m0 * a.lda, a.lda, p.hi - p.m0, a.k);
-  tb.begin(a.w + p.e * a.w_group + (TRB ? (long long)n0 * ES : n0 * a.ldw), a.ldw, a.n - n0, a.k);
+  ta.begin(a.a + (long long)p.m0 * a.lda, a.lda, p.hi - p.m0, a.k, tid);
+  tb.begin(a.b + p.e * a.b_group + (TRB ? (long long)n0 * ES : n0 * a.ldb), a.ldb, a.n - n0, a.k, tid);
   f32x16 acc[MT][NT];
-  C::run(ta, tb, 0, (a.k + C::KST - 1) / C::KST, smem, wm, wn, acc);
+  C::run(ta, tb, 0, (a.k + C::KST - 1) / C::KST, smem, group, wm, wn, acc);
+  if (group > 0) return;
 #pragma unroll
   for (int i = 0; i < MT; ++i) {
     const int m = p.m0 + (wm * MT + i) * 32 + (threadIdx.x & 31);
@@ -164,26 +161,51 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void grouped_rows_kernel(RowsArgs 
   }
 }
 
+// A group's last tile is on average half full.  Half of it or less is multiplied as a tile of half the height.
+template <int ES, bool TRB, int WM, int WN, int MT, int NT, int KG, int DB, bool VEC, bool OUT16>
+__global__ __launch_bounds__(WM * WN * KG * 64, 2) void grouped_rows_kernel(FewArgs a) {
+  typedef Core<ES, false, TRB, WM, WN, MT, NT, KG, DB, VEC> C;
+  __shared__ __attribute__((aligned(1024))) char smem[KG * C::RING];
+  typedef typename std::conditional<OUT16, __bf16, float>::type out_t;
+  const Place p = place_tile<C::BM>(a.offsets, a.groups, a.rows, a.ntiles, blockIdx.x, gridDim.x);
+  if (!p.live) {
+    if (a.clear) clear_rest(p, (out_t*)a.y, a.ldy, a.rows, a.n, C::NTH * KG);
+    return;
+  }
+  const int group = KG == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / C::NTH), tid = threadIdx.x - group * C::NTH;
+  if constexpr (MT > 1) {
+    if (p.hi - p.m0 <= C::BM / 2) {
+      rows_tile<Core<ES, false, TRB, WM, WN, MT / 2, NT, KG, DB, VEC>, TRB, ES, WN, MT / 2, NT, OUT16>(a, p, smem, group, tid);
+      return;
+    }
+  }
+  rows_tile<C, TRB, ES, WN, MT, NT, OUT16>(a, p, smem, group, tid);
+}
+
 // dw_e = dy_e^T . x_e.  Workgroup: group, tile of dw, and a share of the group's rows (whole stages).
-template <int ES, int WM, int WN, int MT, int NT, int D, bool VEC>
-__global__ __launch_bounds__(WM * WN * 64, 2) void grouped_wgrad_kernel(WgradArgs a) {
-  typedef Core<ES, true, true, WM, WN, MT, NT, D, VEC> C;
-  __shared__ __attribute__((aligned(1024))) char smem[D * C::STAGE];
+template <int ES, int WM, int WN, int MT, int NT, int KG, int DB, bool VEC>
+__global__ __launch_bounds__(WM * WN * KG * 64, 2) void grouped_wgrad_kernel(WgradArgs a) {
+  typedef Core<ES, true, true, WM, WN, MT, NT, KG, DB, VEC> C;
+  __shared__ __attribute__((aligned(1024))) char smem[KG * C::RING];
   const int tiles = a.ntiles * a.ktiles;
   const int e = blockIdx.x / (tiles * a.splits), at = blockIdx.x % (tiles * a.splits);
   const int split = at / tiles, nt = at % tiles / a.ktiles, kt = at % a.ktiles;
   const Span g = group_span(a.offsets, a.groups, a.rows, e);
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int group = KG == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / C::NTH), tid = threadIdx.x - group * C::NTH;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / WN, wn = wave % WN;
   const int n0 = nt * C::BM, k0 = kt * C::BN;
   const int all = (g.hi - g.lo + C::KST - 1) / C::KST;
   const int first = (int)((long long)all * split / a.splits), last = (int)((long long)all * (split + 1) / a.splits);
   typename C::TA ta;
   typename C::TB tb;
-  ta.begin(a.dy + g.lo * a.lddy + (long long)n0 * ES, a.lddy, a.n - n0, g.hi - g.lo);
-  tb.begin(a.x + g.lo * a.ldx + (long long)k0 * ES, a.ldx, a.k - k0, g.hi - g.lo);
+  // (the share's end is the operands' end)
+  const int end = min(g.hi - g.lo, last * C::KST);
+  ta.begin(a.dy + g.lo * a.lddy + (long long)n0 * ES, a.lddy, a.n - n0, end, tid);
+  tb.begin(a.x + g.lo * a.ldx + (long long)k0 * ES, a.ldx, a.k - k0, end, tid);
   f32x16 acc[MT][NT];
-  C::run(ta, tb, first, last - first, smem, wm, wn, acc);
+  C::run(ta, tb, first, last - first, smem, group, wm, wn, acc);
+  if (group > 0) return;
   float* const dw = a.dw + ((long long)split * a.groups + e) * a.n * a.k;
 #pragma unroll
   for (int i = 0; i < MT; ++i) {
@@ -204,17 +226,106 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void grouped_wgrad_kernel(WgradArg
   }
 }
 
-bool fits(long long pitch_bytes) { return pitch_bytes > 0 && pitch_bytes <= C2DP_MAX_PITCH; }
+// dw (+)= the sum of the shares' tiles, in their order.
+__global__ __launch_bounds__(256) void join_shares_kernel(const float* __restrict__ parts, float* __restrict__ dw, long long count,
+                                                          int splits, int accumulate) {
+  for (long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 4; i < count; i += (long long)gridDim.x * 1024) {
+    if (i + 4 <= count) {
+      f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+      if (accumulate) __builtin_memcpy(&v, dw + i, 16);
+      for (int s = 0; s < splits; ++s) {
+        f32x4 p;
+        __builtin_memcpy(&p, parts + s * count + i, 16);
+        v += p;
+      }
+      store_at((char*)(dw + i), v);
+    } else {
+      for (long long j = i; j < count; ++j) {
+        float v = accumulate ? dw[j] : 0.0f;
+        for (int s = 0; s < splits; ++s) v += parts[s * count + j];
+        dw[j] = v;
+      }
+    }
+  }
+}
 
-template <int ES, bool TRB, bool VEC, bool OUT16>
-int launch_rows(RowsArgs a, hipStream_t stream) {
-  constexpr int WM = XWM, WN = XWN, MT = XMT, NT = XNT, D = XD;
+// ---- which kernel ----------------------------------------------------------------------------------
+//
+// The one whose estimated time is least, t = rounds of resident workgroups * (us per stage * stages + us per
+// round), a stage 128 bytes of the contraction, with the rates that each was measured at:
+//   rows, bf16                    a round   a stage             measured (us)
+//   256 x 256 tiles                 3.5      1.65 (1.2 in        8192 x 8192 x 8192: 880, in 128 x 128 tiles 1045;
+//                                            one round)           32 groups of 512 x 2048 x 2048: 185, 207
+//   128 x 128, two per CU           3.5      1.0  (0.55 one       8 groups of 512 x 1024 x 1024: 18.6, 256 x 256 25.9,
+//                                            per CU)              64 x 64 31
+//   64 x 64, two K groups           3.0      0.25                 8 groups of 32 x 1024 x 1024: 7.0, 128 x 128 11.7
+//   32 x 32 from registers          2.5      0.29                 (forward alone)
+// Up to 16 rows a group, forward: 16 x 16 from registers.  fp32 is bound by its matrix instructions (a stage of a
+// 64 x 64 tile 0.56, of 128 x 128 1.9 or, two per CU, 3.8) and has no 256 x 256 tiles, which gain 2.5 % on
+// 4096^3 and lose wherever tiles are few (4 groups of 1024 x 416 x 1024: 241 against 42 in 64 x 64 tiles).
+double rounds_of(double tiles, double slots) { return tiles <= slots ? 1.0 : tiles / slots; }
+
+enum Shape { T256, T128, T64, T32, T16 };
+Shape rows_shape(const FewArgs& a, int es, bool forward, bool vec) {
+  const int groups = a.groups < a.rows ? a.groups : a.rows;
+  if (forward && (long long)a.rows <= 16ll * groups) return T16;
+  auto tiles = [&](int side) { return ((double)a.rows / side + 0.4 * groups) * ((a.n + side - 1) / side); };
+  const double stages = ((long long)a.k * es + 127) / 128;
+  const double t256 = tiles(256), t128 = tiles(128);
+  const double us256 = t256 <= 256 ? 1.2 * stages + 3.5 : rounds_of(t256, 256) * (1.65 * stages + 3.5);
+  const double f = es == 4 ? 3.8 : forward ? 1.0 : 1.5;
+  const double us128 = t128 <= 256 ? 0.55 * f * stages + 3.5 : rounds_of(t128, 512) * (f * stages + 3.5);
+  const double us64 = rounds_of(tiles(64), 256) * ((es == 4 ? 0.56 : 0.25) * stages + 3.0);
+  const double us32 = forward ? rounds_of(tiles(32), 256) * (es == 4 ? 0.4 : 0.29) * stages + 2.5 : 1e30;
+  if (es == 2 && vec && us256 <= us128 && us256 <= us64 && us256 <= us32) return T256;
+  if (us128 <= us64 && us128 <= us32) return T128;
+  return us64 <= us32 ? T64 : T32;
+}
+
+// Weight gradient: the same, the rows of a group the contraction, dealt to `splits` workgroups where the tiles of
+// dw are few; a round ends with the tile's way to memory, and splits with the sum over them.
+struct WgradPlan { int side, splits; };
+WgradPlan wgrad_plan(int groups, int rows, int n, int k, int es) {
+  const double stages = ((double)rows / groups * es + 127) / 128, mb = 4e-6 * groups * n * k;
+  WgradPlan best = {64, 1};
+  double least = 1e30;
+  for (int side = es == 2 ? 256 : 128; side >= 64; side /= 2) {
+    const double tiles = (double)groups * ((n + side - 1) / side) * ((k + side - 1) / side);
+    const double slots = side == 128 ? 512 : 256;
+    const double stage = es == 4 ? (side == 128 ? 3.8 : 0.56) : side == 256 ? 1.7 : side == 128 ? 1.2 : 0.27;
+    const double round = side == 256 ? 20 : side == 128 ? 11 : 4;
+    for (int splits = 1; splits <= 32 && 4 * splits <= stages + 3 && (splits == 1 || splits * mb <= 256); splits *= 2) {
+      const double one = side == 128 && tiles * splits <= 256 ? 0.6 : 1.0;  // (one workgroup per CU)
+      const double t = rounds_of(tiles * splits, slots) * one * (stage * stages / splits + round) +
+                       (splits > 1 ? 4.0 + (splits + 1) * mb / 4.0 : 0.0);
+      if (t < least) { least = t; best = {side, splits}; }
+    }
+  }
+  return best;
+}
+
+template <int ES, bool TRB, int WM, int WN, int MT, int NT, int KG, int DB, bool VEC, bool OUT16>
+int launch_tiles(FewArgs a, hipStream_t stream) {
   constexpr int BM = WM * MT * 32, BN = WN * NT * 32;
   a.ntiles = (a.n + BN - 1) / BN;
   const unsigned grid = place_grid(BM, a.groups, true, a.rows, a.ntiles);
   if (!grid) return C2D_ERR_UNSUPPORTED;
-  hipLaunchKernelGGL((grouped_rows_kernel<ES, TRB, WM, WN, MT, NT, D, VEC, OUT16>), dim3(grid), dim3(WM * WN * 64), 0, stream, a);
+  hipLaunchKernelGGL((grouped_rows_kernel<ES, TRB, WM, WN, MT, NT, KG, DB, VEC, OUT16>), dim3(grid), dim3(WM * WN * KG * 64), 0, stream, a);
   return c2d_launch_status();
+}
+
+template <int ES, bool TRB, bool VEC, bool OUT16>
+int launch_rows(const FewArgs& a, hipStream_t stream) {
+  const Shape shape = rows_shape(a, ES, !TRB, VEC);
+  if constexpr (ES == 2 && VEC) {
+    if (shape == T256) return launch_tiles<ES, TRB, 2, 4, 4, 2, 1, 2, true, OUT16>(a, stream);
+  }
+  if constexpr (!TRB) {
+    if (shape == T16) return launch_sixteen_rows<ES == 2 ? BF16 : F32, false, VEC, OUT16>(a, stream);
+    if (shape == T32) return launch_few<ES == 2 ? BF16 : F32, false, 2, 2, 8, VEC, OUT16>(a, stream);
+  }
+  if (shape == T128) return launch_tiles<ES, TRB, 2, 2, 2, 2, 1, 2, VEC, OUT16>(a, stream);
+  return launch_tiles<ES, TRB, 2, 2, 1, 1, 2, 4, VEC, OUT16>(a, stream);
 }
 
 template <bool TRB>
@@ -229,12 +340,12 @@ int rows_product(const void* x, int x_type, long long ldx, const void* w, const 
   const int es = x_type == C2DP_BF16 ? 2 : 4, ys = y_type == C2DP_BF16 ? 2 : 4;
   if ((long long)(contraction > 0 ? ldx : 1) * es > C2DP_MAX_PITCH || (long long)(k > 0 ? k : 1) * es > C2DP_MAX_PITCH)
     return C2D_ERR_UNSUPPORTED;
-  RowsArgs a;
+  FewArgs a = {};
   a.a = (const char*)x;
   a.lda = ldx * es;
-  a.w = (const char*)w;
-  a.ldw = (long long)k * es;
-  a.w_group = (long long)n * contraction * es;
+  a.b = (const char*)w;
+  a.ldb = (long long)k * es;
+  a.b_group = (long long)n * contraction * es;
   a.offsets = offsets;
   a.y = (char*)y;
   a.ldy = ldy;
@@ -245,7 +356,7 @@ int rows_product(const void* x, int x_type, long long ldx, const void* w, const 
   a.clear = clear;
   const hipStream_t s = (hipStream_t)stream;
   // (16-byte loads: the contraction's last chunk is whole; across it, a row of w is whole chunks)
-  const bool vec = aligned16(x, a.lda) && aligned16(w, a.ldw) && (long long)contraction * es % 16 == 0;
+  const bool vec = aligned16(x, a.lda) && aligned16(w, a.ldb) && (long long)contraction * es % 16 == 0;
   if (es == 4) return vec ? launch_rows<4, TRB, true, false>(a, s) : launch_rows<4, TRB, false, false>(a, s);
   if (ys == 4) return vec ? launch_rows<2, TRB, true, false>(a, s) : launch_rows<2, TRB, false, false>(a, s);
   return vec ? launch_rows<2, TRB, true, true>(a, s) : launch_rows<2, TRB, false, true>(a, s);
@@ -267,23 +378,30 @@ extern "C" int c2dp_grouped_matmul_dgrad(const void* dy, int dy_type, long long 
   return rows_product<true>(dy, dy_type, lddy, w, offsets, groups, dx, dx_type, lddx, rows, k, k, n, clear_rest, stream);
 }
 
-extern "C" unsigned long long c2dp_grouped_matmul_wgrad_workspace_bytes(int groups, int rows, int n, int k) {
-  (void)groups; (void)rows; (void)n; (void)k;
-  return 0;
+extern "C" unsigned long long c2dp_grouped_matmul_wgrad_workspace_bytes(int groups, int rows, int n, int k, int x_type) {
+  if (groups <= 0 || rows <= 0 || n <= 0 || k <= 0 || (x_type != C2DP_F32 && x_type != C2DP_BF16)) return 0;
+  const int splits = wgrad_plan(groups, rows, n, k, x_type == C2DP_BF16 ? 2 : 4).splits;
+  return splits > 1 ? 4ull * splits * groups * n * k : 0;
 }
 
 namespace {
-template <int ES, bool VEC>
+template <int ES, int WM, int WN, int MT, int NT, int KG, int DB, bool VEC>
 int launch_wgrad(WgradArgs a, hipStream_t stream) {
-  constexpr int WM = XWM, WN = XWN, MT = XMT, NT = XNT, D = XD;
-  constexpr int BM = WM * MT * 32, BN = WN * NT * 32;
-  a.ntiles = (a.n + BM - 1) / BM;
-  a.ktiles = (a.k + BN - 1) / BN;
-  a.splits = 1;
+  a.ntiles = (a.n + WM * MT * 32 - 1) / (WM * MT * 32);
+  a.ktiles = (a.k + WN * NT * 32 - 1) / (WN * NT * 32);
   const long long grid = (long long)a.groups * a.ntiles * a.ktiles * a.splits;
   if (grid >= (1ll << 30)) return C2D_ERR_UNSUPPORTED;
-  hipLaunchKernelGGL((grouped_wgrad_kernel<ES, WM, WN, MT, NT, D, VEC>), dim3((unsigned)grid), dim3(WM * WN * 64), 0, stream, a);
+  hipLaunchKernelGGL((grouped_wgrad_kernel<ES, WM, WN, MT, NT, KG, DB, VEC>), dim3((unsigned)grid), dim3(WM * WN * KG * 64), 0, stream, a);
   return c2d_launch_status();
+}
+
+template <int ES, bool VEC>
+int launch_wgrad_side(const WgradArgs& a, int side, hipStream_t stream) {
+  if constexpr (ES == 2 && VEC) {
+    if (side == 256) return launch_wgrad<2, 4, 2, 2, 4, 1, 2, true>(a, stream);
+  }
+  if (side >= 128) return launch_wgrad<ES, 2, 2, 2, 2, 1, 2, VEC>(a, stream);
+  return launch_wgrad<ES, 2, 2, 1, 1, 2, 4, VEC>(a, stream);
 }
 }  // namespace
 
@@ -296,22 +414,32 @@ extern "C" int c2dp_grouped_matmul_wgrad(const void* x, int x_type, long long ld
   if (n == 0 || k == 0) return C2D_OK;
   C2D_CHECK_ARG(offsets && dw && (rows == 0 || (x && dy)));
   const int es = x_type == C2DP_BF16 ? 2 : 4;
-  if (!fits(ldx * es) || !fits(lddy * es)) return C2D_ERR_UNSUPPORTED;
-  (void)workspace; (void)workspace_bytes;
+  if (ldx * es > C2DP_MAX_PITCH || lddy * es > C2DP_MAX_PITCH) return C2D_ERR_UNSUPPORTED;
+  const unsigned long long need = c2dp_grouped_matmul_wgrad_workspace_bytes(groups, rows, n, k, x_type);
+  if (workspace_bytes < need || (need && !workspace)) return C2D_ERR_WORKSPACE;
+  C2D_CHECK_ARG(((unsigned long long)workspace & 15) == 0);
+  const WgradPlan plan = wgrad_plan(groups, rows, n, k, es);
   WgradArgs a;
   a.dy = (const char*)dy;
   a.x = (const char*)x;
   a.lddy = lddy * es;
   a.ldx = ldx * es;
   a.offsets = offsets;
-  a.dw = dw;
+  a.splits = need ? plan.splits : 1;
+  a.dw = need ? (float*)workspace : dw;
   a.groups = groups;
   a.rows = rows;
   a.n = n;
   a.k = k;
-  a.accumulate = accumulate;
+  a.accumulate = need ? 0 : accumulate;
   const bool vec = aligned16(x, a.ldx) && aligned16(dy, a.lddy) && n * es % 16 == 0 && k * es % 16 == 0;
   const hipStream_t s = (hipStream_t)stream;
-  if (es == 4) return vec ? launch_wgrad<4, true>(a, s) : launch_wgrad<4, false>(a, s);
-  return vec ? launch_wgrad<2, true>(a, s) : launch_wgrad<2, false>(a, s);
+  const int status = es == 4 ? (vec ? launch_wgrad_side<4, true>(a, plan.side, s) : launch_wgrad_side<4, false>(a, plan.side, s))
+                             : (vec ? launch_wgrad_side<2, true>(a, plan.side, s) : launch_wgrad_side<2, false>(a, plan.side, s));
+  if (status != C2D_OK || !need) return status;
+  const long long count = (long long)groups * n * k;
+  const long long blocks = (count + 1023) / 1024;
+  hipLaunchKernelGGL(join_shares_kernel, dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, s, (const float*)workspace, dw,
+                     count, a.splits, accumulate);
+  return c2d_launch_status();
 }

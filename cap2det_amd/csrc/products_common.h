@@ -41,6 +41,14 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const void* p, long 
                                            0x00020000);
 }
 
+// The same as the four words of a buffer resource.
+__device__ __forceinline__ i32x4 buffer_words(const void* p, long long bytes) {
+  const unsigned long long u = (unsigned long long)p;
+  return i32x4{__builtin_amdgcn_readfirstlane((int)(unsigned)u), __builtin_amdgcn_readfirstlane((int)(unsigned)(u >> 32) & 0xffff),
+               __builtin_amdgcn_readfirstlane((int)(bytes < 0 ? 0 : bytes < (long long)OUTSIDE ? bytes : (long long)OUTSIDE)),
+               0x00020000};
+}
+
 // ---- ragged groups ------------------------------------------------------------------------------
 
 // Group boundaries as they are used: each offset clamped to [0, rows], and at least every earlier one.
@@ -183,14 +191,18 @@ __device__ __forceinline__ void clear_rest(const Place& p, T* y, long long ldy, 
 // LDS image, contraction contiguous: 128-byte rows, 16-byte chunk c of row r at c ^ ((r >> 1) & 7).  A
 // ds_read_b128 takes one chunk of 16 consecutive rows at a time; the XOR puts those on 16 different
 // 16-byte slots of the 256-byte bank period.  TR: 128 / ES rows of R * ES bytes as they lie in memory;
-// bf16 moves 64-byte granule g of row r to g ^ (r & 3), so that the four rows of a transposed read
-// (ds_read_b64_tr_b16) lie on four bank groups.  The image of a load to LDS is lane-linear: the XOR is
+// bf16 moves 64-byte granule g of row r to g ^ (r & 3) (R = 64, two granules a row: g ^ (r >> 1 & 1)), so that
+// the four rows of a transposed read (ds_read_b64_tr_b16) lie on four bank groups.  The image of a load to LDS is lane-linear: the XOR is
 // applied to the address that a lane fetches from.
 //
 // VEC: loads go to LDS directly (buffer_load ... lds, 16 bytes a lane), and lie outside their buffer, which
 // returns zeros, behind the operand's last row and behind the contraction's end.  Not VEC (a pitch, a
 // pointer or a length that 16-byte loads to LDS do not fit): loads to registers, with their own bounds.
-template <int ES, bool TR, int R, int NTH, bool VEC>
+//
+// UNSEEN: the load to LDS is written as an instruction that the compiler does not look into.  It waits for
+// every such load that it knows of before each transposed LDS read, which is the whole latency of the next stage
+// at every step of 16 k (input gradient 8192^3: XXX us, unseen YYY); stage_barrier waits for what is needed.
+template <int ES, bool TR, int R, int NTH, bool VEC, bool UNSEEN = false>
 struct Tile {
   static constexpr int BYTES = R * 128;
   static constexpr int LOADS = BYTES / (NTH * 16);
@@ -205,18 +217,27 @@ struct Tile {
   long long ld;          // bytes
   int across, len;       // rows (TR: columns) from base that exist; contraction elements
   int tid, row, chunk;   // thread among the NTH, its staged row and source chunk of the first pass
+  int wave;              // (of the wave)
   unsigned off;          // its offset; pass i lies i * RPP rows behind it
 
   __device__ __forceinline__ void begin(const void* p, long long ld_bytes, int across_, int len_, int tid_ = threadIdx.x) {
     tid = tid_;
+    wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     base = (const char*)p;
     ld = ld_bytes;
     across = min(across_, R);
     len = len_;
     row = tid / CPR;
     const int pos = tid % CPR;
-    chunk = !TR ? pos ^ ((row >> 1) & 7) : ES == 2 ? pos ^ ((row & 3) << 2) : pos;
+    chunk = pos ^ swizzle(row);
     off = (unsigned)(row * (int)ld + chunk * 16);
+  }
+
+  // what is XORed to the chunk's number in staged row r
+  static __device__ __forceinline__ int swizzle(int r) {
+    if (!TR) return (r >> 1) & 7;
+    if (ES != 2) return 0;
+    return CPR == 8 ? ((r >> 1) & 1) << 2 : (r & 3) << 2;
   }
 
   // Where stage `st` begins, for the passes that follow: (TR) the buffer, else the lane's offset.
@@ -240,11 +261,20 @@ struct Tile {
   // Pass i of stage `st` into LDS at `to`.  (The bound of a buffer holds for lane offset + scalar offset.)
   __device__ __forceinline__ void pass(char* to, const Stage& g, int st, int i) const {
     if constexpr (VEC) {
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"  // (m0 is reserved, and named as overwritten all the same)
 #ifdef __HIP_DEVICE_COMPILE__  // (the host pass refuses 16 bytes here, and with that drops some kernels' stubs)
-      const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(buffer_of(g.base, g.bytes), (lds_void*)(to + i * NTH * 16 + wave * 1024), 16, (int)g.off,
-                                               __builtin_amdgcn_readfirstlane(g.k0 + i * RPP * (int)ld), 0, 0);
+      const int soff = __builtin_amdgcn_readfirstlane(g.k0 + i * RPP * (int)ld);
+      char* const lds = to + i * NTH * 16 + wave * 1024;
+      if constexpr (UNSEEN) {  // (the low half of an LDS pointer is its offset)
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+                     :: "s"(__builtin_amdgcn_readfirstlane((int)(unsigned long long)lds)), "v"(g.off),
+                        "s"(buffer_words(g.base, g.bytes)), "s"(soff) : "memory", "m0");
+      } else {
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(buffer_of(g.base, g.bytes), (lds_void*)lds, 16, (int)g.off, soff, 0, 0);
+      }
 #endif
+#pragma clang diagnostic pop
     } else {
       typedef typename std::conditional<ES == 1, unsigned char,
                                         typename std::conditional<ES == 2, unsigned short, unsigned>::type>::type elem_t;
@@ -283,6 +313,35 @@ __device__ __forceinline__ void stage_barrier() {
 
 // No load to LDS is on its way any more: before the LDS is another workgroup's.
 __device__ __forceinline__ void drain_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+// Adds the sums of KG groups of NTH threads that made the same tile, in the groups' order; group 0 has them then.
+// `sums`: (KG - 1) * NTH * 64 bytes that nobody else uses any more.
+template <int KG, int NTH, int MT, int NT>
+__device__ __forceinline__ void join_groups(float* sums, int group, int tid, f32x16 (&acc)[MT][NT]) {
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      __syncthreads();
+      if (group > 0) {
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          *(f32x4*)&sums[(((group - 1) * 4 + g) * NTH + tid) * 4] =
+              f32x4{acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
+      }
+      __syncthreads();
+      if (group == 0) {
+#pragma unroll
+        for (int o = 0; o < KG - 1; ++o)
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const f32x4 v = *(const f32x4*)&sums[((o * 4 + g) * NTH + tid) * 4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[i][j][4 * g + r] += v[r];
+          }
+      }
+    }
+}
 
 // ---- result -----------------------------------------------------------------------------------------
 

@@ -1070,7 +1070,7 @@ def grouped_matmul_wgrad(x, dy, offsets, out=None, accumulate=False):
     _whole(dw, "out", _WIDE_TYPES[:1], (groups, n, k), device)
     _given_result(dw, (groups, n, k), _WIDE_TYPES[:1], device, (x, dy, offsets))
   if groups and n and k:
-    nbytes = _wgrad_workspace_bytes(groups, rows, n, k)
+    nbytes = _wgrad_workspace_bytes(groups, rows, n, k, _PRODUCT_TYPE[x.dtype])
     ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
     _lib.call("c2dp_grouped_matmul_wgrad", x.data_ptr(), _PRODUCT_TYPE[x.dtype], _pitch(x, "x"), dy.data_ptr(),
               _pitch(dy, "dy"), offsets.data_ptr(), groups, dw.data_ptr(), rows, n, k, 1 if accumulate else 0,
@@ -1079,5 +1079,5 @@ def grouped_matmul_wgrad(x, dy, offsets, out=None, accumulate=False):
 
 
 @functools.lru_cache(maxsize=1024)
-def _wgrad_workspace_bytes(groups, rows, n, k):
-  return int(_lib.load().c2dp_grouped_matmul_wgrad_workspace_bytes(groups, rows, n, k))
+def _wgrad_workspace_bytes(groups, rows, n, k, kind):
+  return int(_lib.load().c2dp_grouped_matmul_wgrad_workspace_bytes(groups, rows, n, k, kind))

@@ -82,7 +82,7 @@ int c2dp_grouped_matmul_dgrad(const void* dy, int dy_type, long long lddy, const
  *   x [rows][k] pitch ldx;  dy [rows][n] pitch lddy;  dw [groups][n][k] contiguous
  *   workspace: c2dp_grouped_matmul_wgrad_workspace_bytes(...) bytes, 16-byte aligned (may be NULL when that is
  *   0); its contents need not be set, and calls that may run at the same time need one each. */
-unsigned long long c2dp_grouped_matmul_wgrad_workspace_bytes(int groups, int rows, int n, int k);
+unsigned long long c2dp_grouped_matmul_wgrad_workspace_bytes(int groups, int rows, int n, int k, int x_type);
 int c2dp_grouped_matmul_wgrad(const void* x, int x_type, long long ldx, const void* dy, long long lddy,
                               const int32_t* offsets, int groups, float* dw, int rows, int n, int k,
                               int accumulate, void* workspace, unsigned long long workspace_bytes,
