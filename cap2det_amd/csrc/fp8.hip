@@ -256,17 +256,17 @@ __device__ __forceinline__ f32x16 fp8_half(const i32x4 (&b)[4], const i32x4 (&a)
   }
 }
 
-// The stages of B go round DB buffers, those of A round DB + 1: while a stage is multiplied, the next of B and
-// the next two of A are on their way (DB = 2).  Within a stage the loads are issued between the matrix
+// The stages of A go round D buffers, those of B round D + 1: while a stage is multiplied, the next of A and
+// the next two of B are on their way (D = 2; five buffers are what the LDS holds of 256 x 256 tiles).  Within a stage the loads are issued between the matrix
 // instructions of its first tiles, and a tile's scaling runs under the matrix instructions of the next.
 //
 // KG > 1: KG groups of WM x WN waves share the tile, group g taking the stages g, g + KG, ..; their sums are
 // joined through LDS, in the groups' order.  A stage of a small tile is a chain of waits (barrier, LDS read, two
 // matrix instructions, scaling) of 0.5 us whatever its size (64 x 64 tiles): where there is a workgroup per CU
 // or less, KG chains run side by side (256 x 4096 x 4096: 17.6 us, with two groups 13.6, with four 14.6).
-template <bool E5M2, int WM, int WN, int MT, int NT, int KG, int DB, bool VEC>
+template <bool E5M2, int WM, int WN, int MT, int NT, int KG, int D, bool VEC>
 struct Fp8Tiles {
-  static constexpr int BM = WM * MT * 32, BN = WN * NT * 32, NTH = WM * WN * 64, DA = DB + 1, TILES = MT * NT;
+  static constexpr int BM = WM * MT * 32, BN = WN * NT * 32, NTH = WM * WN * 64, DA = D, DB = D + 1, TILES = MT * NT;
   typedef Tile<1, false, BM, NTH, VEC> TA;
   typedef Tile<1, false, BN, NTH, VEC> TB;
   static constexpr int PASSES = TA::LOADS + TB::LOADS;
@@ -276,10 +276,10 @@ struct Fp8Tiles {
 };
 
 // A row tile (`p`) of BM rows or less.
-template <bool E5M2, int WM, int WN, int MT, int NT, int KG, int DB, bool VEC, bool OUT16>
+template <bool E5M2, int WM, int WN, int MT, int NT, int KG, int D, bool VEC, bool OUT16>
 __device__ __forceinline__ void fp8_tile(const FewArgs& a, const Place& p, char* smem, int group, int tid) {
-  typedef Fp8Tiles<E5M2, WM, WN, MT, NT, KG, DB, VEC> C;
-  constexpr int BN = C::BN, NTH = C::NTH, DA = C::DA, TILES = C::TILES, PASSES = C::PASSES, RING = C::RING;
+  typedef Fp8Tiles<E5M2, WM, WN, MT, NT, KG, D, VEC> C;
+  constexpr int BN = C::BN, NTH = C::NTH, DA = C::DA, DB = C::DB, TILES = C::TILES, PASSES = C::PASSES, RING = C::RING;
   typedef typename C::TA TA;
   typedef typename C::TB TB;
   typedef typename std::conditional<OUT16, __bf16, float>::type out_t;
@@ -320,17 +320,17 @@ __device__ __forceinline__ void fp8_tile(const FewArgs& a, const Place& p, char*
   };
   if (rounds > 0) {
     load_scales(group);
-    ta.issue(ring_a, group);
+    tb.issue(ring_b, group);
 #pragma unroll
-    for (int d = 0; d < DB - 1; ++d) {
-      tb.issue(ring_b + d * TB::BYTES, d * KG + group);
-      ta.issue(ring_a + (d + 1) * TA::BYTES, (d + 1) * KG + group);
+    for (int d = 0; d < D - 1; ++d) {
+      ta.issue(ring_a + d * TA::BYTES, d * KG + group);
+      tb.issue(ring_b + (d + 1) * TB::BYTES, (d + 1) * KG + group);
     }
   }
   int now_a = 0, now_b = 0, next_a = DA - 1, next_b = DB - 1;
   for (int it = 0; it < rounds; ++it) {
-    // (behind this stage's B have been issued: A of the next, and DB - 2 whole stages)
-    stage_barrier<VEC, TA::LOADS + (DB - 2) * PASSES>();
+    // (behind this stage's A have been issued: B of the next, and D - 2 whole stages)
+    stage_barrier<VEC, TB::LOADS + (D - 2) * PASSES>();
     float scale[MT];
 #pragma unroll
     for (int i = 0; i < MT; ++i) scale[i] = KG > 1 && col_scale == 0.0f ? 0.0f : row_scale[i] * col_scale;
@@ -371,8 +371,8 @@ __device__ __forceinline__ void fp8_tile(const FewArgs& a, const Place& p, char*
       }
 #pragma unroll
       for (int q = u * PER; q < (u + 1) * PER && q < PASSES; ++q) {
-        if (q < TB::LOADS) tb.pass(ring_b + next_b * TB::BYTES, gb, st_b, q);
-        else ta.pass(ring_a + next_a * TA::BYTES, ga, st_a, q - TB::LOADS);
+        if (q < TA::LOADS) ta.pass(ring_a + next_a * TA::BYTES, ga, st_a, q);
+        else tb.pass(ring_b + next_b * TB::BYTES, gb, st_b, q - TA::LOADS);
       }
     }
     now_a = now_a + 1 == DA ? 0 : now_a + 1;
@@ -383,37 +383,38 @@ __device__ __forceinline__ void fp8_tile(const FewArgs& a, const Place& p, char*
   drain_loads();
   if constexpr (KG > 1) {
     join_groups<KG, NTH>((float*)smem, group, tid, acc);
-    if (group > 0) return;
   }
 #pragma unroll
   for (int j = 0; j < NT; ++j) {
-    const int n = n0 + (wn * NT + j) * 32;
     float add[16];
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-      const int c = n + 8 * (r >> 2) + 4 * lh + (r & 3);
+      const int c = n0 + (wn * NT + j) * 32 + 8 * (r >> 2) + 4 * lh + (r & 3);
       add[r] = a.bias && c < a.n ? a.bias[(long long)p.e * a.n + c] : 0.0f;
     }
 #pragma unroll
-    for (int i = 0; i < MT; ++i) {
-      const int m = p.m0 + (wm * MT + i) * 32 + li;
+    for (int i = 0; i < MT; ++i)
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const float v = acc[i][j][r] + add[r];
         acc[i][j][r] = a.relu && v < 0.0f ? 0.0f : v;
       }
-      store_tile<OUT16>(acc[i][j], m < p.hi && n < a.n ? (char*)((out_t*)a.y + m * a.ldy + n) : nullptr, a.n - n);
-    }
   }
+  __syncthreads();
+  if (group > 0) return;
+  typedef Store<OUT16, NT> S;
+  static_assert(NTH / 64 * S::BYTES <= RING, "the result goes out through the ring's LDS");
+  const int m = p.m0 + wm * MT * 32, n = n0 + wn * NT * 32;
+  S::run(acc, smem + wave * S::BYTES, (char*)((out_t*)a.y + m * a.ldy + n), a.ldy * (long long)sizeof(out_t), p.hi - m, a.n - n);
 }
 
 // A group's last tile is on average half full.  Half of it or less is multiplied as a tile of half the height.
-template <bool E5M2, int WM, int WN, int MT, int NT, int KG, int DB, bool VEC, bool OUT16>
+template <bool E5M2, int WM, int WN, int MT, int NT, int KG, int D, bool VEC, bool OUT16>
 __global__ __launch_bounds__(WM * WN * KG * 64, 2) void fp8_tile_kernel(FewArgs a) {
-  typedef Fp8Tiles<E5M2, WM, WN, MT, NT, KG, DB, VEC> C;
+  typedef Fp8Tiles<E5M2, WM, WN, MT, NT, KG, D, VEC> C;
   __shared__ __attribute__((aligned(1024))) char smem[KG * C::RING];
   typedef typename std::conditional<OUT16, __bf16, float>::type out_t;
-  const Place p = place_tile<C::BM>(a.offsets, a.groups, a.rows, a.ntiles, blockIdx.x, gridDim.x);
+  const Place p = place_tile<C::BM, (MT > 1)>(a.offsets, a.groups, a.rows, a.ntiles, blockIdx.x, gridDim.x, a.slots);
   if (!p.live) {
     if (a.clear) clear_rest(p, (out_t*)a.y, a.ldy, a.rows, a.n, C::NTH * KG);
     return;
@@ -421,20 +422,21 @@ __global__ __launch_bounds__(WM * WN * KG * 64, 2) void fp8_tile_kernel(FewArgs 
   const int group = KG == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / C::NTH), tid = threadIdx.x - group * C::NTH;
   if constexpr (MT > 1) {
     if (p.hi - p.m0 <= C::BM / 2) {
-      fp8_tile<E5M2, WM, WN, MT / 2, NT, KG, DB, VEC, OUT16>(a, p, smem, group, tid);
+      fp8_tile<E5M2, WM, WN, MT / 2, NT, KG, D, VEC, OUT16>(a, p, smem, group, tid);
       return;
     }
   }
-  fp8_tile<E5M2, WM, WN, MT, NT, KG, DB, VEC, OUT16>(a, p, smem, group, tid);
+  fp8_tile<E5M2, WM, WN, MT, NT, KG, D, VEC, OUT16>(a, p, smem, group, tid);
 }
 
-template <bool E5M2, int WM, int WN, int MT, int NT, int KG, int DB, bool VEC, bool OUT16>
+template <bool E5M2, int WM, int WN, int MT, int NT, int KG, int D, bool VEC, bool OUT16>
 int launch_tiles(FewArgs a, hipStream_t stream) {
   constexpr int BM = WM * MT * 32, BN = WN * NT * 32;
   a.ntiles = (a.n + BN - 1) / BN;
-  const unsigned grid = place_grid(BM, a.groups, a.offsets != nullptr, a.rows, a.ntiles);
+  a.slots = slots_per_xcd(KG * Fp8Tiles<E5M2, WM, WN, MT, NT, KG, D, VEC>::RING);
+  const unsigned grid = place_grid(BM, a.groups, a.offsets != nullptr, a.rows, a.ntiles, MT > 1 ? a.slots / 2 : 0);
   if (!grid) return C2D_ERR_UNSUPPORTED;
-  hipLaunchKernelGGL((fp8_tile_kernel<E5M2, WM, WN, MT, NT, KG, DB, VEC, OUT16>), dim3(grid), dim3(WM * WN * KG * 64), 0, stream, a);
+  hipLaunchKernelGGL((fp8_tile_kernel<E5M2, WM, WN, MT, NT, KG, D, VEC, OUT16>), dim3(grid), dim3(WM * WN * KG * 64), 0, stream, a);
   return c2d_launch_status();
 }
 

@@ -15,14 +15,16 @@ struct WgradArgs {
   int ntiles, ktiles, splits, accumulate;
 };
 
-// The stages of B go round DB buffers, those of A round DB + 1: while a stage is multiplied, the next of B and
-// the next two of A are on their way (DB = 2; two of each and a half are what the LDS holds of 256 x 256 tiles, and
-// a load takes longer than a stage).  One barrier per stage; the loads are issued between the matrix instructions of
-// its first half, since a burst of them behind the barrier holds up every wave of the workgroup.
+// The stages of A go round D buffers, those of B round D + 1: while a stage is multiplied, the next of A and
+// the next two of B are on their way (D = 2; five buffers are what the LDS holds of 256 x 256 tiles, and a load takes
+// longer than a stage).  B are the weights, which come from memory, each group's own, where rows come from L2
+// for all but one of their column tiles (32 groups of about 512 x 2048 x 2048: XXX us, with the third buffer A's YYY).
+// One barrier per stage; the loads are issued between the matrix instructions of its first half, since a burst
+// of them behind the barrier holds up every wave of the workgroup.
 // KG > 1: KG groups of WM x WN waves share the tile, group g taking the stages g, g + KG, ..
-template <int ES, bool TRA, bool TRB, int WM, int WN, int MT, int NT, int KG, int DB, bool VEC>
+template <int ES, bool TRA, bool TRB, int WM, int WN, int MT, int NT, int KG, int D, bool VEC>
 struct Core {
-  static constexpr int BM = WM * MT * 32, BN = WN * NT * 32, NTH = WM * WN * 64, DA = DB + 1;
+  static constexpr int BM = WM * MT * 32, BN = WN * NT * 32, NTH = WM * WN * 64, DA = D, DB = D + 1;
   typedef Tile<ES, TRA, BM, NTH, VEC, TRA || TRB> TA;
   typedef Tile<ES, TRB, BN, NTH, VEC, TRA || TRB> TB;
   static constexpr int RING = DA * TA::BYTES + DB * TB::BYTES;
@@ -79,24 +81,24 @@ struct Core {
     char* const ring_b = ring_a + DA * TA::BYTES;
     const int rounds = (stages + KG - 1) / KG;
     // (a stage behind the last reads zeros: the operands end there)
-    ta.issue(ring_a, first + group);
+    tb.issue(ring_b, first + group);
 #pragma unroll
-    for (int d = 0; d < DB - 1; ++d) {
-      tb.issue(ring_b + d * TB::BYTES, first + d * KG + group);
-      ta.issue(ring_a + (d + 1) * TA::BYTES, first + (d + 1) * KG + group);
+    for (int d = 0; d < D - 1; ++d) {
+      ta.issue(ring_a + d * TA::BYTES, first + d * KG + group);
+      tb.issue(ring_b + (d + 1) * TB::BYTES, first + (d + 1) * KG + group);
     }
     int now_a = 0, now_b = 0, next_a = DA - 1, next_b = DB - 1;
     for (int it = 0; it < rounds; ++it) {
-      // (behind this stage's B have been issued: A of the next, and DB - 2 whole stages)
-      stage_barrier<VEC, TA::LOADS + (DB - 2) * PASSES>();
+      // (behind this stage's A have been issued: B of the next, and D - 2 whole stages)
+      stage_barrier<VEC, TB::LOADS + (D - 2) * PASSES>();
       const int st_a = first + (it + DA - 1) * KG + group, st_b = first + (it + DB - 1) * KG + group;
       const typename TA::Stage ga = ta.at(st_a);
       const typename TB::Stage gb = tb.at(st_b);
       const char* const sa = ring_a + now_a * TA::BYTES;
       const char* const sb = ring_b + now_b * TB::BYTES;
       auto pass = [&](int q) {
-        if (q < TB::LOADS) tb.pass(ring_b + next_b * TB::BYTES, gb, st_b, q);
-        else ta.pass(ring_a + next_a * TA::BYTES, ga, st_a, q - TB::LOADS);
+        if (q < TA::LOADS) ta.pass(ring_a + next_a * TA::BYTES, ga, st_a, q);
+        else tb.pass(ring_b + next_b * TB::BYTES, gb, st_b, q - TA::LOADS);
       };
       constexpr int QS = ES == 2 ? 1 : 4, SLOTS = 4 * QS * MT * NT;  // matrix instructions of a stage
       constexpr int PER = (2 * PASSES + SLOTS - 1) / SLOTS, EVERY = PER > 1 ? 1 : SLOTS / (2 * PASSES);
@@ -149,25 +151,21 @@ __device__ __forceinline__ void rows_tile(const FewArgs& a, const Place& p, char
   tb.begin(a.b + p.e * a.b_group + (TRB ? (long long)n0 * ES : n0 * a.ldb), a.ldb, a.n - n0, a.k, tid);
   f32x16 acc[MT][NT];
   C::run(ta, tb, 0, (a.k + C::KST - 1) / C::KST, smem, group, wm, wn, acc);
+  __syncthreads();
   if (group > 0) return;
-#pragma unroll
-  for (int i = 0; i < MT; ++i) {
-    const int m = p.m0 + (wm * MT + i) * 32 + (threadIdx.x & 31);
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      const int n = n0 + (wn * NT + j) * 32;
-      store_tile<OUT16>(acc[i][j], m < p.hi && n < a.n ? (char*)((out_t*)a.y + m * a.ldy + n) : nullptr, a.n - n);
-    }
-  }
+  typedef Store<OUT16, NT> S;
+  static_assert(C::NTH / 64 * S::BYTES <= C::RING, "the result goes out through the ring's LDS");
+  const int m = p.m0 + wm * MT * 32, n = n0 + wn * NT * 32;
+  S::run(acc, smem + wave * S::BYTES, (char*)((out_t*)a.y + m * a.ldy + n), a.ldy * (long long)sizeof(out_t), p.hi - m, a.n - n);
 }
 
 // A group's last tile is on average half full.  Half of it or less is multiplied as a tile of half the height.
-template <int ES, bool TRB, int WM, int WN, int MT, int NT, int KG, int DB, bool VEC, bool OUT16>
+template <int ES, bool TRB, int WM, int WN, int MT, int NT, int KG, int D, bool VEC, bool OUT16>
 __global__ __launch_bounds__(WM * WN * KG * 64, 2) void grouped_rows_kernel(FewArgs a) {
-  typedef Core<ES, false, TRB, WM, WN, MT, NT, KG, DB, VEC> C;
+  typedef Core<ES, false, TRB, WM, WN, MT, NT, KG, D, VEC> C;
   __shared__ __attribute__((aligned(1024))) char smem[KG * C::RING];
   typedef typename std::conditional<OUT16, __bf16, float>::type out_t;
-  const Place p = place_tile<C::BM>(a.offsets, a.groups, a.rows, a.ntiles, blockIdx.x, gridDim.x);
+  const Place p = place_tile<C::BM, (MT > 1)>(a.offsets, a.groups, a.rows, a.ntiles, blockIdx.x, gridDim.x, a.slots);
   if (!p.live) {
     if (a.clear) clear_rest(p, (out_t*)a.y, a.ldy, a.rows, a.n, C::NTH * KG);
     return;
@@ -175,7 +173,7 @@ __global__ __launch_bounds__(WM * WN * KG * 64, 2) void grouped_rows_kernel(FewA
   const int group = KG == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / C::NTH), tid = threadIdx.x - group * C::NTH;
   if constexpr (MT > 1) {
     if (p.hi - p.m0 <= C::BM / 2) {
-      rows_tile<Core<ES, false, TRB, WM, WN, MT / 2, NT, KG, DB, VEC>, TRB, ES, WN, MT / 2, NT, OUT16>(a, p, smem, group, tid);
+      rows_tile<Core<ES, false, TRB, WM, WN, MT / 2, NT, KG, D, VEC>, TRB, ES, WN, MT / 2, NT, OUT16>(a, p, smem, group, tid);
       return;
     }
   }
@@ -183,9 +181,9 @@ __global__ __launch_bounds__(WM * WN * KG * 64, 2) void grouped_rows_kernel(FewA
 }
 
 // dw_e = dy_e^T . x_e.  Workgroup: group, tile of dw, and a share of the group's rows (whole stages).
-template <int ES, int WM, int WN, int MT, int NT, int KG, int DB, bool VEC>
+template <int ES, int WM, int WN, int MT, int NT, int KG, int D, bool VEC>
 __global__ __launch_bounds__(WM * WN * KG * 64, 2) void grouped_wgrad_kernel(WgradArgs a) {
-  typedef Core<ES, true, true, WM, WN, MT, NT, KG, DB, VEC> C;
+  typedef Core<ES, true, true, WM, WN, MT, NT, KG, D, VEC> C;
   __shared__ __attribute__((aligned(1024))) char smem[KG * C::RING];
   const int tiles = a.ntiles * a.ktiles;
   const int e = blockIdx.x / (tiles * a.splits), at = blockIdx.x % (tiles * a.splits);
@@ -205,25 +203,13 @@ __global__ __launch_bounds__(WM * WN * KG * 64, 2) void grouped_wgrad_kernel(Wgr
   tb.begin(a.x + g.lo * a.ldx + (long long)k0 * ES, a.ldx, a.k - k0, end, tid);
   f32x16 acc[MT][NT];
   C::run(ta, tb, first, last - first, smem, group, wm, wn, acc);
+  __syncthreads();
   if (group > 0) return;
-  float* const dw = a.dw + ((long long)split * a.groups + e) * a.n * a.k;
-#pragma unroll
-  for (int i = 0; i < MT; ++i) {
-    const int n = n0 + (wm * MT + i) * 32 + (threadIdx.x & 31);
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      const int k = k0 + (wn * NT + j) * 32;
-      float* const row = n < a.n && k < a.k ? dw + (long long)n * a.k + k : nullptr;
-      if (a.accumulate && row) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int c = 8 * (r >> 2) + 4 * ((threadIdx.x >> 5) & 1) + (r & 3);
-          if (k + c < a.k) acc[i][j][r] += row[c];
-        }
-      }
-      store_tile<false>(acc[i][j], (char*)row, a.k - k);
-    }
-  }
+  typedef Store<false, NT> S;
+  static_assert(C::NTH / 64 * S::BYTES <= C::RING, "the result goes out through the ring's LDS");
+  const int n = n0 + wm * MT * 32, k = k0 + wn * NT * 32;
+  float* const dw = a.dw + ((long long)split * a.groups + e) * a.n * a.k + (long long)n * a.k + k;
+  S::run(acc, smem + wave * S::BYTES, (char*)dw, a.k * 4ll, a.n - n, a.k - k, a.accumulate);
 }
 
 // dw (+)= the sum of the shares' tiles, in their order.
@@ -254,10 +240,12 @@ __global__ __launch_bounds__(256) void join_shares_kernel(const float* __restric
 // The one whose estimated time is least, t = rounds of resident workgroups * (us per stage * stages + us per
 // round), a stage 128 bytes of the contraction, with the rates that each was measured at:
 //   rows, bf16                    a round   a stage             measured (us)
-//   256 x 256 tiles                 3.5      1.65 (1.2 in        8192 x 8192 x 8192: 880, in 128 x 128 tiles 1045;
-//                                            one round)           32 groups of 512 x 2048 x 2048: 185, 207
+//   256 x 256 tiles                 3.5      1.65 (1.2 in        8192 x 8192 x 8192: 851, in 128 x 128 tiles 1045;
+//                                            one round)           32 groups of 512 x 2048 x 2048: 177, 207
 //   128 x 128, two per CU           3.5      1.0  (0.55 one       8 groups of 512 x 1024 x 1024: 18.6, 256 x 256 25.9,
 //                                            per CU)              64 x 64 31
+//     input gradient                3.5      1.55 (0.55)         8 groups of 625 x 1000 x 1536: 34, 256 x 256 29;
+//                                                                8 groups of 512 x 1024 x 1024: 19.4, 256 x 256 27
 //   64 x 64, two K groups           3.0      0.25                 8 groups of 32 x 1024 x 1024: 7.0, 128 x 128 11.7
 //   32 x 32 from registers          2.5      0.29                 (forward alone)
 // Up to 16 rows a group, forward: 16 x 16 from registers.  fp32 is bound by its matrix instructions (a stage of a
@@ -272,9 +260,10 @@ Shape rows_shape(const FewArgs& a, int es, bool forward, bool vec) {
   auto tiles = [&](int side) { return ((double)a.rows / side + 0.4 * groups) * ((a.n + side - 1) / side); };
   const double stages = ((long long)a.k * es + 127) / 128;
   const double t256 = tiles(256), t128 = tiles(128);
-  const double us256 = t256 <= 256 ? 1.2 * stages + 3.5 : rounds_of(t256, 256) * (1.65 * stages + 3.5);
-  const double f = es == 4 ? 3.8 : forward ? 1.0 : 1.5;
-  const double us128 = t128 <= 256 ? 0.55 * f * stages + 3.5 : rounds_of(t128, 512) * (f * stages + 3.5);
+  const double us256 = t256 <= 256 ? (forward ? 1.2 : 1.5) * stages + 3.5 : rounds_of(t256, 256) * (1.65 * stages + 3.5);
+  // (128 x 128: from one workgroup per CU to two)
+  const double one = es == 4 ? 1.9 : 0.55, two = es == 4 ? 3.8 : forward ? 1.0 : 1.55;
+  const double us128 = rounds_of(t128, 512) * ((t128 <= 256 ? one : t128 >= 512 ? two : one + (two - one) * (t128 - 256) / 256) * stages + 3.5);
   const double us64 = rounds_of(tiles(64), 256) * ((es == 4 ? 0.56 : 0.25) * stages + 3.0);
   const double us32 = forward ? rounds_of(tiles(32), 256) * (es == 4 ? 0.4 : 0.29) * stages + 2.5 : 1e30;
   if (es == 2 && vec && us256 <= us128 && us256 <= us64 && us256 <= us32) return T256;
@@ -304,13 +293,14 @@ WgradPlan wgrad_plan(int groups, int rows, int n, int k, int es) {
   return best;
 }
 
-template <int ES, bool TRB, int WM, int WN, int MT, int NT, int KG, int DB, bool VEC, bool OUT16>
+template <int ES, bool TRB, int WM, int WN, int MT, int NT, int KG, int D, bool VEC, bool OUT16>
 int launch_tiles(FewArgs a, hipStream_t stream) {
   constexpr int BM = WM * MT * 32, BN = WN * NT * 32;
   a.ntiles = (a.n + BN - 1) / BN;
-  const unsigned grid = place_grid(BM, a.groups, true, a.rows, a.ntiles);
+  a.slots = slots_per_xcd(KG * Core<ES, false, TRB, WM, WN, MT, NT, KG, D, VEC>::RING);
+  const unsigned grid = place_grid(BM, a.groups, true, a.rows, a.ntiles, MT > 1 ? a.slots / 2 : 0);
   if (!grid) return C2D_ERR_UNSUPPORTED;
-  hipLaunchKernelGGL((grouped_rows_kernel<ES, TRB, WM, WN, MT, NT, KG, DB, VEC, OUT16>), dim3(grid), dim3(WM * WN * KG * 64), 0, stream, a);
+  hipLaunchKernelGGL((grouped_rows_kernel<ES, TRB, WM, WN, MT, NT, KG, D, VEC, OUT16>), dim3(grid), dim3(WM * WN * KG * 64), 0, stream, a);
   return c2d_launch_status();
 }
 
@@ -385,13 +375,13 @@ extern "C" unsigned long long c2dp_grouped_matmul_wgrad_workspace_bytes(int grou
 }
 
 namespace {
-template <int ES, int WM, int WN, int MT, int NT, int KG, int DB, bool VEC>
+template <int ES, int WM, int WN, int MT, int NT, int KG, int D, bool VEC>
 int launch_wgrad(WgradArgs a, hipStream_t stream) {
   a.ntiles = (a.n + WM * MT * 32 - 1) / (WM * MT * 32);
   a.ktiles = (a.k + WN * NT * 32 - 1) / (WN * NT * 32);
   const long long grid = (long long)a.groups * a.ntiles * a.ktiles * a.splits;
   if (grid >= (1ll << 30)) return C2D_ERR_UNSUPPORTED;
-  hipLaunchKernelGGL((grouped_wgrad_kernel<ES, WM, WN, MT, NT, KG, DB, VEC>), dim3((unsigned)grid), dim3(WM * WN * KG * 64), 0, stream, a);
+  hipLaunchKernelGGL((grouped_wgrad_kernel<ES, WM, WN, MT, NT, KG, D, VEC>), dim3((unsigned)grid), dim3(WM * WN * KG * 64), 0, stream, a);
   return c2d_launch_status();
 }
 

@@ -101,48 +101,73 @@ struct Place {
 
 // Tile of workgroup `bid` out of `nbid` (a multiple of 8).  The host cannot know how many row tiles the
 // groups make; it launches the largest number, rows / BM + groups, and each wave counts them here: one
-// or two loads and a dozen lane shuffles for 64 groups.  Workgroups go round the 8 XCDs by number; XCD x
+// or two loads and two dozen lane shuffles for 64 groups.  Workgroups go round the 8 XCDs by number; XCD x
 // takes the x-th eighth of the tiles, in bands of 4 row tiles by all column tiles, so that what
 // runs there at a time shares rows and weights in that XCD's L2.
-template <int BM>
+// HALVES: a tile of BM / 2 rows or less costs half, and a group's last one often is.  All of those come behind the
+// others; and where the others end with a round that would leave most of an XCD's `slots` resident
+// workgroups without a tile, the tiles of that round are made as halves too (32 groups of about 512 x 2048 x 2048:
+// XXX us, in the groups' order YYY).
+template <int BM, bool HALVES>
 __device__ __forceinline__ Place place_tile(const int* __restrict__ offsets, int groups, int rows, int ntiles,
-                                            unsigned bid, unsigned nbid) {
+                                            unsigned bid, unsigned nbid, int slots) {
   Place p;
-  int mtiles = 0, carry = 0;
+  int carry = 0, full = 0, half = 0;  // row tiles of all groups
   Span s = {0, rows};
-  int upto = 0;
+  auto fulls = [](int r) { return HALVES ? (r + BM / 2 - 1) / BM : (r + BM - 1) / BM; };
+  auto halves = [&](int r) { return (r + BM - 1) / BM - fulls(r); };
+  int upto_full = 0, upto_half = 0;
   if (!offsets) {
-    mtiles = (rows + BM - 1) / BM;
+    full = (rows + BM - 1) / BM;
     p.begin = 0;
     p.end = rows;
   } else {
     for (int base = 0; base < groups; base += 64) {
       s = lane_span(offsets, groups, rows, base, &carry);
       if (base == 0) p.begin = __builtin_amdgcn_readlane(s.lo, 0);
-      upto = lane_prefix_sum((s.hi - s.lo + BM - 1) / BM);
-      mtiles += __builtin_amdgcn_readlane(upto, 63);
+      upto_full = lane_prefix_sum(fulls(s.hi - s.lo));
+      full += __builtin_amdgcn_readlane(upto_full, 63);
+      if (HALVES) {
+        upto_half = lane_prefix_sum(halves(s.hi - s.lo));
+        half += __builtin_amdgcn_readlane(upto_half, 63);
+      }
     }
     p.end = carry;
   }
-  const int tiles = mtiles * ntiles;
   const int xcd = bid & 7, local = bid >> 3, per = nbid >> 3;
-  const int q = tiles >> 3, r = tiles & 7;
-  const int count = q + (xcd < r ? 1 : 0);
-  p.live = local < count;
-  p.spares = 8 * (per - q - (r ? 1 : 0));
+  const int full_tiles = full * ntiles, half_tiles = half * ntiles;
+  const int my_full = (full_tiles + 7 - xcd) >> 3, my_half = (half_tiles + xcd) >> 3;
+  const int over = my_full % slots;
+  const int cut = HALVES && my_full > slots && 2 * over + my_half <= slots ? over : 0;
+  p.live = local < my_full + cut + my_half;
+  p.spares = 8 * (per - ((full_tiles + 7) >> 3) - ((half_tiles + 7) >> 3) - (HALVES ? slots / 2 : 0));
   p.spare = -1;
   if (!p.live) {
-    if (8 * (local - count) + xcd < p.spares) p.spare = 8 * (local - count) + xcd;
+    const int spare = 8 * (local - my_full - cut - my_half) + xcd;
+    if (spare < p.spares) p.spare = spare;
     return p;
   }
-  const int idx = xcd * q + min(xcd, r) + local;
+  // the tile among those of its kind: whole eighths before this XCD's, of which the first (last) few have one more
+  const bool small = HALVES && local >= my_full + cut;
+  const bool halved = local >= my_full - cut && !small && cut > 0;
+  const int nth = small ? local - my_full - cut : halved ? my_full - cut + ((local - my_full + cut) >> 1) : local;
+  const bool second = halved && ((local - my_full + cut) & 1);
+  const int idx = small ? xcd * (half_tiles >> 3) + max(0, xcd - 8 + (half_tiles & 7)) + nth
+                        : xcd * (full_tiles >> 3) + min(xcd, full_tiles & 7) + nth;
   constexpr int BAND = 4;
+  const int mtiles = small ? half : full;
   const int band = idx / (BAND * ntiles), at = idx - band * BAND * ntiles;
   const int bm = min(BAND, mtiles - band * BAND);
   const int mt = band * BAND + at % bm;
   p.nt = at / bm;
+  auto halve = [&] {
+    if (second) p.m0 += BM / 2;
+    else if (halved) p.hi = min(p.hi, p.m0 + BM / 2);
+    p.live = p.m0 < p.hi;
+  };
   if (!offsets) {
     p.e = 0; p.lo = 0; p.hi = rows; p.m0 = mt * BM;
+    halve();
     return p;
   }
   int before = 0;
@@ -150,16 +175,19 @@ __device__ __forceinline__ Place place_tile(const int* __restrict__ offsets, int
   for (int base = 0;; base += 64) {
     if (groups > 64) {
       s = lane_span(offsets, groups, rows, base, &carry);
-      upto = lane_prefix_sum((s.hi - s.lo + BM - 1) / BM);
+      upto_full = lane_prefix_sum(fulls(s.hi - s.lo));
+      if (HALVES) upto_half = lane_prefix_sum(halves(s.hi - s.lo));
     }
+    const int upto = small ? upto_half : upto_full;
     const unsigned long long has = __ballot(before + upto > mt);
     if (has) {
       const int l = __builtin_ctzll(has);
       p.e = base + l;
       p.lo = __builtin_amdgcn_readlane(s.lo, l);
       p.hi = __builtin_amdgcn_readlane(s.hi, l);
-      const int mine = (p.hi - p.lo + BM - 1) / BM;
-      p.m0 = p.lo + (mt - (before + __builtin_amdgcn_readlane(upto, l) - mine)) * BM;
+      const int mine = fulls(p.hi - p.lo);
+      p.m0 = p.lo + (small ? mine : mt - (before + __builtin_amdgcn_readlane(upto, l) - mine)) * BM;
+      halve();
       return p;
     }
     before += __builtin_amdgcn_readlane(upto, 63);
@@ -167,9 +195,10 @@ __device__ __forceinline__ Place place_tile(const int* __restrict__ offsets, int
 }
 
 // The largest number of workgroups that place_tile can need, with some to spare that clear rows; 0: too many.
-inline unsigned place_grid(int BM, int groups, bool ragged, int rows, int ntiles) {
+// `cut`: tiles of an XCD that may be made as halves.
+inline unsigned place_grid(int BM, int groups, bool ragged, int rows, int ntiles, int cut) {
   const long long mt = ragged ? (long long)rows / BM + (groups < rows ? groups : rows) : ((long long)rows + BM - 1) / BM;
-  const long long n = ((mt * ntiles + 7) / 8 + (ragged ? 8 : 0)) * 8;
+  const long long n = ((mt * ntiles + 7) / 8 + cut + (ragged ? 8 : 0)) * 8;
   return n < (1ll << 30) ? (unsigned)n : 0u;
 }
 
@@ -356,49 +385,66 @@ __device__ __forceinline__ unsigned pack_bf16(float a, float b) {
 template <class V>
 __device__ __forceinline__ void store_at(char* p, V v) { __builtin_memcpy(p, &v, sizeof(V)); }
 
-// A 32 x 32 result tile: lane l holds row m = l & 31, register r column 8 (r >> 2) + 4 (l >> 5) + (r & 3).
-// fp32: four 16-byte stores of 4 columns.  bf16: the halves of the wave exchange registers
-// (v_permlane32_swap) so that each holds 8 consecutive columns, two 16-byte stores.  `row`: this lane's row
-// of the result at the tile's first column, null if there is none; `cols`: columns that exist.
-template <bool BF16>
-__device__ __forceinline__ void store_tile(const f32x16& v, char* row, int cols) {
-  const int lh = (threadIdx.x >> 5) & 1;
-  if constexpr (BF16) {
-    unsigned w[8];
+// A wave's MT x NT result tiles of 32 x 32: lane l holds row m = l & 31, register r column 8 (r >> 2) + 4 (l >> 5) +
+// (r & 3).  They go to memory through LDS, 32 rows at a time, so that a store writes whole rows of the wave's
+// columns, 16 bytes a lane: straight from the registers an instruction would write 32 bytes of each of 32
+// rows (weight gradient of 32 groups of 2048 x 2048: XXX us, straight YYY).
+//   lds   LDS that nobody else uses any more, STORE_BYTES a wave
+//   y     the wave's first row and column of the result, pitch ldy bytes; `rows`, `cols`: how many exist
+//   add   the result is added to what is there (fp32)
+template <bool BF16, int NT>
+struct Store {
+  static constexpr int ES = BF16 ? 2 : 4, ROW = NT * 32 * ES, PITCH = ROW + 16, BYTES = 32 * PITCH;
+  static constexpr int LANES = ROW / 16, STEP = 64 / LANES;  // lanes a row, rows an instruction
+
+  template <int MT>
+  static __device__ __forceinline__ void run(const f32x16 (&acc)[MT][NT], char* lds, char* y, long long ldy, int rows, int cols,
+                                             bool add = false) {
+    const int lane = threadIdx.x & 63, li = lane & 31, lh = lane >> 5;
+    const int col = (lane % LANES) * (16 / ES);
 #pragma unroll
-    for (int g = 0; g < 8; ++g) w[g] = pack_bf16(v[2 * g], v[2 * g + 1]);
+    for (int i = 0; i < MT; ++i) {
+      if (i * 32 >= rows) break;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      // w[4h..4h+1]: columns 16h + 4 lh ..; w[4h+2..4h+3]: columns 16h + 8 + 4 lh ..
-      const auto x = __builtin_amdgcn_permlane32_swap(w[4 * h], w[4 * h + 2], false, false);
-      const auto y = __builtin_amdgcn_permlane32_swap(w[4 * h + 1], w[4 * h + 3], false, false);
-      const u32x4 o = {x[0], y[0], x[1], y[1]};  // columns 16 h + 8 lh .. + 7
-      const int c = 16 * h + 8 * lh;
-      if (row) {
-        if (c + 8 <= cols) {
-          store_at(row + c * 2, o);
-        } else {
+      for (int j = 0; j < NT; ++j)
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if (c + j < cols) ((unsigned short*)row)[c + j] = (unsigned short)(o[j >> 1] >> (16 * (j & 1)));
+        for (int g = 0; g < 4; ++g) {
+          char* const to = lds + li * PITCH + (j * 32 + 8 * g + 4 * lh) * ES;
+          const f32x16& v = acc[i][j];
+          if constexpr (BF16) *(u32x2*)to = u32x2{pack_bf16(v[4 * g], v[4 * g + 1]), pack_bf16(v[4 * g + 2], v[4 * g + 3])};
+          else *(f32x4*)to = f32x4{v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]};
         }
-      }
-    }
-  } else {
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const int c = 8 * g + 4 * lh;
-      if (row) {
-        if (c + 4 <= cols) {
-          store_at(row + c * 4, f32x4{v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]});
-        } else {
+      for (int t = 0; t < 32 / STEP; ++t) {
+        const int r = t * STEP + lane / LANES, m = i * 32 + r;
+        u32x4 v = *(const u32x4*)(lds + r * PITCH + col * ES);
+        if (m < rows && col < cols) {
+          char* const to = y + m * ldy + (long long)col * ES;
+          if (col + 16 / ES <= cols) {
+            if (!BF16 && add) {
+              f32x4 old;
+              __builtin_memcpy(&old, to, 16);
+              v = __builtin_bit_cast(u32x4, __builtin_bit_cast(f32x4, v) + old);
+            }
+            store_at(to, v);
+          } else {
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (c + j < cols) ((float*)row)[c + j] = v[4 * g + j];
+            for (int e = 0; e < 16 / ES; ++e)
+              if (col + e < cols) {
+                if constexpr (BF16) ((unsigned short*)to)[e] = (unsigned short)(v[e >> 1] >> (16 * (e & 1)));
+                else ((float*)to)[e] = __uint_as_float(v[e]) + (add ? ((const float*)to)[e] : 0.0f);
+              }
+          }
         }
       }
     }
   }
+};
+
+// Workgroups with this much LDS that an XCD of this process holds at a time.
+inline int slots_per_xcd(int lds_bytes) {
+  const int n = c2d_available_cus() / 8 * (160 * 1024 / lds_bytes);
+  return n > 0 ? n : 1;
 }
 
 inline bool aligned16(const void* p, long long pitch_bytes) {
