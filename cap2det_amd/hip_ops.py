@@ -918,6 +918,20 @@ def _given_result(out, shape, types, device, operands):
         raise ValueError("out: shares memory with an operand")
 
 
+# Each call below asks first, in one expression, whether its arguments are as they usually are (a sixth of a call's
+# time on the host, asked one by one a third); what is not goes through the checks that name what is wrong, and
+# through _pitch.
+
+_F32, _BF16, _E4M3 = torch.float32, torch.bfloat16, torch.float8_e4m3fn
+
+
+def _tensors(*ts):
+  for t in ts:
+    if not isinstance(t, torch.Tensor):
+      return False
+  return True
+
+
 def fp8_quantize(x, block_rows=1, dtype=torch.float8_e4m3fn):
   """8-bit values and fp32 scales of a matrix, or of a stack of matrices: x [.., rows, cols] fp32 or bf16 ->
   (q [.., rows, cols], scale [.., ceil(rows / block_rows), ceil(cols / 128)]), x ~ q * scale of its block.
@@ -926,7 +940,8 @@ def fp8_quantize(x, block_rows=1, dtype=torch.float8_e4m3fn):
   2^-126, F = 448 (float8_e4m3fn) or 57344 (float8_e5m2); q = x / scale in fp32, to the nearest, ties to
   even.  A NaN stays one and takes no part in the maximum, an infinity makes its block's values NaN.
   The blocks of a weight matrix w are square: q.t().contiguous() and scale.t().contiguous() are w.t()'s."""
-  _operand(x, "x", _WIDE_TYPES, 3 if isinstance(x, torch.Tensor) and x.dim() == 3 else 2, _device())
+  if not (isinstance(x, torch.Tensor) and x.get_device() == _device() and x.dtype in _WIDE_TYPES and x.dim() == 2):
+    _operand(x, "x", _WIDE_TYPES, 3 if isinstance(x, torch.Tensor) and x.dim() == 3 else 2, _device())
   if dtype not in FP8_TYPES:
     raise ValueError("dtype: one of %s is wanted, got %s" % (_names(FP8_TYPES), dtype))
   if block_rows != 1 and block_rows != FP8_BLOCK:
@@ -940,32 +955,49 @@ def fp8_quantize(x, block_rows=1, dtype=torch.float8_e4m3fn):
     batch, step = shape[0], x.stride(0)
     ld = _pitch(x[0], "x") if batch else cols
     grid = (batch,) + grid
-  q = torch.empty(shape, dtype=dtype, device=x.device)
-  scale = torch.empty(grid, dtype=torch.float32, device=x.device)
+  q = x.new_empty(shape, dtype=dtype)
+  scale = x.new_empty(grid, dtype=_F32)
   if batch and rows and cols:
     _lib.call("c2dp_fp8_quantize", x.data_ptr(), _PRODUCT_TYPE[x.dtype], ld, step, q.data_ptr(), _PRODUCT_TYPE[dtype],
               scale.data_ptr(), batch, rows, cols, block_rows, _stream())
   return q, scale
 
 
-def _fp8_product(a, a_scale, b, b_scale, offsets, groups, n, k, out, out_dtype, bias, relu, device):
-  rows = a.shape[0]
+def _check_fp8(a, a_scale, b, b_scale, offsets, bias, dense):
+  """Names what is wrong with the operands of an 8-bit product."""
+  device = _device()
+  _operand(a, "a", FP8_TYPES, 2, device)
+  _operand(b, "b", FP8_TYPES[:1], 2 if dense else 3, device)
+  lead = tuple(b.shape[:-2])
+  n, k = b.shape[-2:]
+  if not dense and lead[0] == 0:
+    raise ValueError("b: at least one group is wanted, got shape %s" % (tuple(b.shape),))
   if a.shape[1] != k:
     raise ValueError("a: %d columns are wanted, got shape %s" % (k, tuple(a.shape)))
+  kb, nb = -(-k // FP8_BLOCK), -(-n // FP8_BLOCK)
+  _whole(b, "b", FP8_TYPES, lead + (n, k), device)
+  _whole(a_scale, "a_scale", (_F32,), (a.shape[0], kb), device)
+  _whole(b_scale, "b_scale", (_F32,), lead + (nb, kb), device)
+  if not dense:
+    _whole(offsets, "offsets", (torch.int32,), (lead[0] + 1,), device)
+  if bias is not None:
+    _whole(bias, "bias", (_F32,), lead + (n,), device)
+
+
+def _fp8_product(a, a_scale, b, b_scale, offsets, groups, rows, n, k, out, out_dtype, bias, relu):
   if out is None:
-    if out_dtype not in _WIDE_TYPES:
+    if out_dtype is not _BF16 and out_dtype is not _F32:
       raise ValueError("out_dtype: one of %s is wanted, got %s" % (_names(_WIDE_TYPES), out_dtype))
-    y = torch.empty((rows, n), dtype=out_dtype, device=a.device)
-    ldy = n
+    y, ldy, clear = a.new_empty((rows, n), dtype=out_dtype), n, 1
   else:
-    y = out
-    _given_result(y, (rows, n), _WIDE_TYPES, device, (a, a_scale, b, b_scale, bias, offsets))
+    y, clear = out, 0
+    _given_result(y, (rows, n), _WIDE_TYPES, _device(), (a, a_scale, b, b_scale, bias, offsets))
     ldy = _pitch(y, "out")
   if rows and n:
     _lib.call("c2dp_fp8_matmul", a.data_ptr(), _PRODUCT_TYPE[a.dtype], _pitch(a, "a"), a_scale.data_ptr(), b.data_ptr(),
               b_scale.data_ptr(), None if offsets is None else offsets.data_ptr(), groups,
               None if bias is None else bias.data_ptr(), 1 if relu else 0, y.data_ptr(), _PRODUCT_TYPE[y.dtype], ldy,
-              rows, n, k, 1 if out is None else 0, _stream())
+              rows, n, k, clear, _stream())
   return y
 
 
@@ -975,38 +1007,35 @@ def fp8_matmul(a, a_scale, b, b_scale, out=None, out_dtype=torch.bfloat16, bias=
   [n, k] float8_e4m3fn with b_scale [ceil(n / 128), ceil(k / 128)] (block_rows 128), bias [n] fp32 ->
   [rows, n] bf16 or fp32.  The input gradient is the same product on the transposed weight."""
   device = _device()
-  _operand(a, "a", FP8_TYPES, 2, device)
-  _operand(b, "b", FP8_TYPES[:1], 2, device)
+  if not (bias is None and _tensors(a, a_scale, b, b_scale) and a.dim() == 2 and b.dim() == 2 and
+          a.get_device() == b.get_device() == a_scale.get_device() == b_scale.get_device() == device and
+          a.dtype in FP8_TYPES and b.dtype is _E4M3 and a_scale.dtype is b_scale.dtype is _F32 and a.shape[1] == b.shape[1] and
+          a_scale.shape == (a.shape[0], -(-b.shape[1] // FP8_BLOCK)) and
+          b_scale.shape == (-(-b.shape[0] // FP8_BLOCK), -(-b.shape[1] // FP8_BLOCK)) and
+          b.is_contiguous() and a_scale.is_contiguous() and b_scale.is_contiguous()):
+    _check_fp8(a, a_scale, b, b_scale, None, bias, True)
   n, k = b.shape
-  kb = -(-k // FP8_BLOCK)
-  _whole(b, "b", FP8_TYPES, (n, k), device)
-  _whole(a_scale, "a_scale", _WIDE_TYPES[:1], (a.shape[0], kb), device)
-  _whole(b_scale, "b_scale", _WIDE_TYPES[:1], (-(-n // FP8_BLOCK), kb), device)
-  if bias is not None:
-    _whole(bias, "bias", _WIDE_TYPES[:1], (n,), device)
-  return _fp8_product(a, a_scale, b, b_scale, None, 1, n, k, out, out_dtype, bias, relu, device)
+  return _fp8_product(a, a_scale, b, b_scale, None, 1, a.shape[0], n, k, out, out_dtype, bias, relu)
 
 
 def grouped_matmul_fp8(a, a_scale, b, b_scale, offsets, out=None, out_dtype=torch.bfloat16, bias=None, relu=False):
   """fp8_matmul with one weight matrix per group of rows: b [groups, n, k], b_scale [groups, ceil(n / 128),
   ceil(k / 128)], bias [groups, n]."""
   device = _device()
-  _operand(a, "a", FP8_TYPES, 2, device)
-  _operand(b, "b", FP8_TYPES[:1], 3, device)
+  if not (bias is None and _tensors(a, a_scale, b, b_scale, offsets) and a.dim() == 2 and b.dim() == 3 and b.shape[0] > 0 and
+          a.get_device() == b.get_device() == a_scale.get_device() == b_scale.get_device() == offsets.get_device() == device and
+          a.dtype in FP8_TYPES and b.dtype is _E4M3 and a_scale.dtype is b_scale.dtype is _F32 and
+          offsets.dtype is torch.int32 and offsets.shape == (b.shape[0] + 1,) and a.shape[1] == b.shape[2] and
+          a_scale.shape == (a.shape[0], -(-b.shape[2] // FP8_BLOCK)) and
+          b_scale.shape == (b.shape[0], -(-b.shape[1] // FP8_BLOCK), -(-b.shape[2] // FP8_BLOCK)) and
+          b.is_contiguous() and a_scale.is_contiguous() and b_scale.is_contiguous() and offsets.is_contiguous()):
+    _check_fp8(a, a_scale, b, b_scale, offsets, bias, False)
   groups, n, k = b.shape
-  if groups == 0:
-    raise ValueError("b: at least one group is wanted, got shape %s" % (tuple(b.shape),))
-  kb = -(-k // FP8_BLOCK)
-  _whole(b, "b", FP8_TYPES, (groups, n, k), device)
-  _whole(a_scale, "a_scale", _WIDE_TYPES[:1], (a.shape[0], kb), device)
-  _whole(b_scale, "b_scale", _WIDE_TYPES[:1], (groups, -(-n // FP8_BLOCK), kb), device)
-  _whole(offsets, "offsets", (torch.int32,), (groups + 1,), device)
-  if bias is not None:
-    _whole(bias, "bias", _WIDE_TYPES[:1], (groups, n), device)
-  return _fp8_product(a, a_scale, b, b_scale, offsets, groups, n, k, out, out_dtype, bias, relu, device)
+  return _fp8_product(a, a_scale, b, b_scale, offsets, groups, a.shape[0], n, k, out, out_dtype, bias, relu)
 
 
-def _grouped_rows(entry, x, name, w, offsets, out, out_dtype, dgrad):
+def _check_grouped(x, name, w, offsets, dgrad):
+  """Names what is wrong with the operands of a grouped product."""
   device = _device()
   _operand(x, name, _WIDE_TYPES, 2, device)
   _operand(w, "w", (x.dtype,), 3, device)
@@ -1015,23 +1044,34 @@ def _grouped_rows(entry, x, name, w, offsets, out, out_dtype, dgrad):
     raise ValueError("w: at least one group is wanted, got shape %s" % (tuple(w.shape),))
   _whole(w, "w", (x.dtype,), (groups, n, k), device)
   _whole(offsets, "offsets", (torch.int32,), (groups + 1,), device)
-  rows, cols, wide = x.shape[0], n if dgrad else k, k if dgrad else n
+  cols = n if dgrad else k
   if x.shape[1] != cols:
     raise ValueError("%s: %d columns are wanted, got shape %s" % (name, cols, tuple(x.shape)))
-  types = _WIDE_TYPES if x.dtype == torch.bfloat16 else _WIDE_TYPES[:1]
+
+
+def _grouped_rows(entry, x, name, w, offsets, out, out_dtype, dgrad):
+  if not (_tensors(x, w, offsets) and x.dim() == 2 and w.dim() == 3 and w.shape[0] > 0 and
+          x.get_device() == w.get_device() == offsets.get_device() == _device() and w.dtype is x.dtype and
+          x.dtype in _WIDE_TYPES and offsets.dtype is torch.int32 and offsets.shape == (w.shape[0] + 1,) and
+          x.shape[1] == w.shape[1 if dgrad else 2] and w.is_contiguous() and offsets.is_contiguous()):
+    _check_grouped(x, name, w, offsets, dgrad)
+  groups, n, k = w.shape
+  rows, wide = x.shape[0], k if dgrad else n
   if out is None:
-    out_dtype = out_dtype or x.dtype
-    if out_dtype not in types:
-      raise ValueError("out_dtype: one of %s is wanted, got %s" % (_names(types), out_dtype))
-    y = torch.empty((rows, wide), dtype=out_dtype, device=x.device)
-    ldy = wide
+    if out_dtype is None or out_dtype is x.dtype:
+      y = x.new_empty((rows, wide))
+    elif out_dtype is _F32:
+      y = x.new_empty((rows, wide), dtype=_F32)
+    else:
+      raise ValueError("out_dtype: %s or %s for operands of %s, got %s" % (_F32, x.dtype, x.dtype, out_dtype))
+    ldy, clear = wide, 1
   else:
-    y = out
-    _given_result(y, (rows, wide), types, device, (x, w, offsets))
+    y, clear = out, 0
+    _given_result(y, (rows, wide), _WIDE_TYPES if x.dtype is _BF16 else (_F32,), _device(), (x, w, offsets))
     ldy = _pitch(y, "out")
   if rows and wide:
     _lib.call(entry, x.data_ptr(), _PRODUCT_TYPE[x.dtype], _pitch(x, name), w.data_ptr(), offsets.data_ptr(), groups,
-              y.data_ptr(), _PRODUCT_TYPE[y.dtype], ldy, rows, n, k, 1 if out is None else 0, _stream())
+              y.data_ptr(), _PRODUCT_TYPE[y.dtype], ldy, rows, n, k, clear, _stream())
   return y
 
 
@@ -1046,32 +1086,39 @@ def grouped_matmul_dgrad(dy, w, offsets, out=None, out_dtype=None):
   return _grouped_rows("c2dp_grouped_matmul_dgrad", dy, "dy", w, offsets, out, out_dtype, True)
 
 
-def grouped_matmul_wgrad(x, dy, offsets, out=None, accumulate=False):
-  """Weight gradient of grouped_matmul: x [rows, k], dy [rows, n] -> dw [groups, n, k] fp32, dw_e =
-  dy_e^T . x_e, zero for an empty group; accumulate=True adds that to `out`.  The same call gives the same
-  bits."""
+def _check_wgrad(x, dy, offsets):
   device = _device()
   _operand(x, "x", _WIDE_TYPES, 2, device)
   _operand(dy, "dy", (x.dtype,), 2, device)
   _operand(offsets, "offsets", (torch.int32,), 1, device)
-  rows, k = x.shape
-  n, groups = dy.shape[1], offsets.numel() - 1
-  if dy.shape[0] != rows:
-    raise ValueError("dy: %d rows are wanted, got shape %s" % (rows, tuple(dy.shape)))
-  if groups < 1:
+  if dy.shape[0] != x.shape[0]:
+    raise ValueError("dy: %d rows are wanted, got shape %s" % (x.shape[0], tuple(dy.shape)))
+  if offsets.numel() < 2:
     raise ValueError("offsets: at least two numbers are wanted, got %d" % offsets.numel())
-  _whole(offsets, "offsets", (torch.int32,), (groups + 1,), device)
+  _whole(offsets, "offsets", (torch.int32,), tuple(offsets.shape), device)
+
+
+def grouped_matmul_wgrad(x, dy, offsets, out=None, accumulate=False):
+  """Weight gradient of grouped_matmul: x [rows, k], dy [rows, n] -> dw [groups, n, k] fp32, dw_e =
+  dy_e^T . x_e, zero for an empty group; accumulate=True adds that to `out`.  The same call gives the same
+  bits."""
+  if not (_tensors(x, dy, offsets) and x.dim() == 2 and dy.dim() == 2 and offsets.dim() == 1 and offsets.shape[0] > 1 and
+          x.get_device() == dy.get_device() == offsets.get_device() == _device() and dy.dtype is x.dtype and
+          x.dtype in _WIDE_TYPES and offsets.dtype is torch.int32 and dy.shape[0] == x.shape[0] and offsets.is_contiguous()):
+    _check_wgrad(x, dy, offsets)
+  rows, k = x.shape
+  n, groups = dy.shape[1], offsets.shape[0] - 1
   if out is None:
     if accumulate:
       raise ValueError("accumulate: there is no `out` to add to")
-    dw = torch.empty((groups, n, k), dtype=torch.float32, device=x.device)
+    dw = x.new_empty((groups, n, k), dtype=_F32)
   else:
     dw = out
-    _whole(dw, "out", _WIDE_TYPES[:1], (groups, n, k), device)
-    _given_result(dw, (groups, n, k), _WIDE_TYPES[:1], device, (x, dy, offsets))
-  if groups and n and k:
+    _whole(dw, "out", (_F32,), (groups, n, k), _device())
+    _given_result(dw, (groups, n, k), (_F32,), _device(), (x, dy, offsets))
+  if n and k:
     nbytes = _wgrad_workspace_bytes(groups, rows, n, k, _PRODUCT_TYPE[x.dtype])
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
+    ws = x.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
     _lib.call("c2dp_grouped_matmul_wgrad", x.data_ptr(), _PRODUCT_TYPE[x.dtype], _pitch(x, "x"), dy.data_ptr(),
               _pitch(dy, "dy"), offsets.data_ptr(), groups, dw.data_ptr(), rows, n, k, 1 if accumulate else 0,
               None if ws is None else ws.data_ptr(), nbytes, _stream())
