@@ -839,7 +839,8 @@ def x9_planes(t):
 # Groups of rows are given by `offsets`, an int32 device tensor of groups + 1 row numbers: group e owns
 # the rows offsets[e] .. offsets[e + 1] - 1 and may be empty.  Nothing here reads them on the host.  An offset
 # outside [0, rows] counts as the nearer end, one below an earlier one as that one.  Rows in no group are
-# not read; in a result they are zero, or, where `out` is given, left as they were.
+# not read; in a result they are zero, or, where `out` is given, left as they were.  `out` has to lie outside the
+# memory that the operands span, gaps between their rows included.
 #
 # Matrices may be row-strided views (columns contiguous).  Everything is queued on the current stream of the
 # current device, where the tensors have to be; results and workspaces of one call are the call's own, so

@@ -157,7 +157,7 @@ def _want(a, a_scale, b, b_scale, bias=None, relu=False):
 
 SIZES = [(1, 1, 1), (1, 16, 128), (3, 129, 16), (16, 128, 256), (17, 33, 144), (130, 257, 384), (128, 128, 128), (300, 40, 1000),
          (5, 70, 33), (64, 200, 2048), (33, 1000, 528), (200, 300, 130), (1, 300, 4096), (2, 513, 1552), (40, 96, 8192),
-         (257, 512, 640), (513, 260, 256)]
+         (257, 512, 640), (513, 260, 256), (4100, 4096, 528), (5800, 2048, 256), (2000, 2000, 264)]
 
 
 @pytest.mark.parametrize("a_type", [E4M3, E5M2])
@@ -193,6 +193,17 @@ def test_grouped_products_of_integers_are_exact(a_type, n, k, counts):
   ops.grouped_matmul_fp8(a, a_s, b, b_s, _offs(offsets), out=out, bias=bias, relu=True)
   want[:2], want[offsets[-1]:] = 5.0, 5.0
   assert torch.equal(out, want.float())
+
+
+def test_large_grouped_tiles_of_integers_are_exact():
+  """256 x 256 tiles over ragged groups: last tiles short and long, and a last round that is made as halves."""
+  gen = _gen(31)
+  for counts, n, k in (([3000, 100, 5900, 0, 256], 2048, 400), ([5800], 2048, 512), ([700, 130, 385] * 8, 4096, 256)):
+    offsets = up.offsets_of(counts)
+    a, a_s, b, b_s = _operands(gen, offsets[-1], n, k, E4M3, len(counts))
+    got = ops.grouped_matmul_fp8(a, a_s, b, b_s, _offs(offsets))
+    for e, (lo, hi) in enumerate(up.spans(offsets, offsets[-1])):
+      assert torch.equal(got[lo:hi], _want(a[lo:hi], a_s[lo:hi], b[e], b_s[e]).to(BF16))
 
 
 @pytest.mark.parametrize("a_type", [E4M3, E5M2])

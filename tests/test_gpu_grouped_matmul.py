@@ -73,6 +73,91 @@ def test_larger_products_of_integers_are_exact(dtype, counts, n, k):
   _same(ops.grouped_matmul_wgrad(x, dy, offs), up.grouped_dw(x, dy, offsets))
 
 
+# Sizes at which the estimated times choose 256 x 256 tiles, with groups whose last tile is short, long and whole, more
+# row tiles than an XCD holds at a time, and (5800 rows of 2048 columns) a last round that is made as halves
+@pytest.mark.parametrize("counts,n,k", [([3000, 100, 5900], 2048, 1024), ([5800], 2048, 1024), ([600, 0, 130, 256, 2000, 385] * 2, 1100, 1032)])
+def test_large_tiles_of_integers_are_exact(counts, n, k):
+  gen = _gen(21)
+  offsets = up.offsets_of(counts, first=5)
+  t = offsets[-1] + 40
+  x, dy = up.integers(gen, (t, k), 4, BF16), up.integers(gen, (t, n), 4, BF16)
+  w = up.integers(gen, (len(counts), n, k), 4, BF16)
+  offs, rows = _offs(offsets), up.spans(offsets, t)
+  for got, want in ((ops.grouped_matmul(x, w, offs), up.grouped(x, w, offsets)),
+                    (ops.grouped_matmul(x, w, offs, out_dtype=F32), up.grouped(x, w, offsets)),
+                    (ops.grouped_matmul_dgrad(dy, w, offs), up.grouped(dy, w.transpose(1, 2), offsets))):
+    _same(got, want, rows)
+    assert (got[:5] == 0).all() and (got[offsets[-1]:] == 0).all()
+  _same(ops.grouped_matmul_wgrad(x, dy, offs), up.grouped_dw(x, dy, offsets))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("counts,n,k", [([8192], 512, 512), ([4000, 0, 1], 136, 264), ([3001], 65, 131), ([1000, 1, 2000, 700], 2048, 2048)])
+def test_wgrad_of_long_groups_and_few_tiles(dtype, counts, n, k):
+  """The rows of a group dealt to several workgroups (and, last, 256 x 256 tiles): exact, and added to what is there."""
+  gen = _gen(22)
+  offsets = up.offsets_of(counts)
+  x, dy = up.integers(gen, (offsets[-1], k), 4, dtype), up.integers(gen, (offsets[-1], n), 4, dtype)
+  want = up.grouped_dw(x, dy, offsets)
+  _same(ops.grouped_matmul_wgrad(x, dy, _offs(offsets)), want)
+  start = up.integers(gen, want.shape, 50)
+  out = start.clone()
+  ops.grouped_matmul_wgrad(x, dy, _offs(offsets), out=out, accumulate=True)
+  _same(out, want + start.double())
+
+
+def test_two_graphs_and_two_streams_share_no_workspace():
+  """Weight gradients that take a workspace, captured twice and replayed beside each other and beside eager calls."""
+  gen = _gen(23)
+  offs = _offs([0, 8192])
+  sets = []
+  for _ in range(2):
+    x = torch.randn(8192, 256, generator=gen, device="cuda").to(BF16)
+    dy = torch.randn(8192, 192, generator=gen, device="cuda").to(BF16)
+    out = torch.empty(1, 192, 256, device="cuda")
+    want = ops.grouped_matmul_wgrad(x, dy, offs)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+      ops.grouped_matmul_wgrad(x, dy, offs, out=out)
+    sets.append((x, dy, out, want, graph, torch.cuda.Stream()))
+  for _ in range(5):
+    torch.cuda.synchronize()
+    eager = []
+    for x, dy, out, want, graph, stream in sets:
+      out.fill_(NAN)
+      stream.wait_stream(torch.cuda.current_stream())
+      with torch.cuda.stream(stream):
+        graph.replay()
+        eager.append(ops.grouped_matmul_wgrad(x, dy, offs))
+    torch.cuda.synchronize()
+    for (x, dy, out, want, graph, stream), again in zip(sets, eager):
+      assert torch.equal(out, want) and torch.equal(again, want)
+
+
+def test_a_step_plan_replays_the_products_on_other_tensors():
+  from cap2det_amd.step_plan import StepPlan
+  gen = _gen(24)
+  offs = _offs([0, 30, 30, 100])
+  x, dy = torch.randn(100, 72, generator=gen, device="cuda").to(BF16), torch.randn(100, 40, generator=gen, device="cuda").to(BF16)
+  w = torch.randn(3, 40, 72, generator=gen, device="cuda").to(BF16)
+  y, dx, dw = torch.empty(100, 40, device="cuda", dtype=BF16), torch.empty(100, 72, device="cuda", dtype=BF16), torch.empty(3, 40, 72, device="cuda")
+  plan = StepPlan()
+  plan.bind_tensor("x", x)
+  plan.bind_tensor("dy", dy)
+  with plan.recording():
+    _layer(x, dy, w, offs, y, dx, dw)
+  assert plan.calls == 3
+  for _ in range(3):
+    x2, dy2 = torch.randn_like(x), torch.randn_like(dy)
+    for t in (y, dx, dw):
+      t.fill_(NAN)
+    plan.replay(dict(x=x2, dy=dy2), {})
+    torch.cuda.synchronize()
+    for got, want in zip((y, dx, dw), (ops.grouped_matmul(x2, w, offs), ops.grouped_matmul_dgrad(dy2, w, offs),
+                                       ops.grouped_matmul_wgrad(x2, dy2, offs))):
+      assert torch.equal(got, want)
+
+
 @pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("counts,n,k", [([100, 0, 37], 200, 328), ([9, 3, 1, 0], 96, 640)])
 def test_real_values_within_the_rounding_of_sums(dtype, counts, n, k):
