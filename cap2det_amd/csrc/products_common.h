@@ -54,6 +54,22 @@ __device__ __forceinline__ i32x4 buffer_words(const void* p, long long bytes) {
 // Group boundaries as they are used: each offset clamped to [0, rows], and at least every earlier one.
 struct Span { int lo, hi; };
 
+// Running sums / maxima (of numbers from 0) over the lanes of a wave: four steps within 16 lanes and two across them, as
+// operands of the vector instructions (DPP).  As shuffles through LDS they were most of a workgroup's start.
+template <class Op>
+__device__ __forceinline__ int lane_scan(int v, Op op) {
+  v = op(v, __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false));  // row_shr:1
+  v = op(v, __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false));  // row_shr:2
+  v = op(v, __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false));  // row_shr:4
+  v = op(v, __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false));  // row_shr:8
+  v = op(v, __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false));  // row_bcast:15, into rows 1 and 3
+  v = op(v, __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false));  // row_bcast:31, into rows 2 and 3
+  return v;
+}
+__device__ __forceinline__ int lane_prefix_sum(int v) {
+  return lane_scan(v, [](int a, int b) { return a + b; });
+}
+
 // The spans of groups base .. base + 63, one per lane (empty behind the last group); `carry`: the
 // largest boundary so far, updated.
 __device__ __forceinline__ Span lane_span(const int* __restrict__ offsets, int groups, int rows, int base,
@@ -61,24 +77,10 @@ __device__ __forceinline__ Span lane_span(const int* __restrict__ offsets, int g
   const int i = base + (int)(threadIdx.x & 63);
   int lo = max(0, min(rows, offsets[min(i, groups)]));
   const int next = max(0, min(rows, offsets[min(i + 1, groups)]));
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int o = __shfl_up(lo, d, 64);
-    if ((int)(threadIdx.x & 63) >= d) lo = max(lo, o);
-  }
-  lo = max(lo, *carry);
+  lo = max(lane_scan(lo, [](int a, int b) { return max(a, b); }), *carry);
   const int hi = max(lo, next);
   *carry = __builtin_amdgcn_readlane(hi, 63);
   return {lo, i < groups ? hi : lo};
-}
-
-__device__ __forceinline__ int lane_prefix_sum(int v) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int o = __shfl_up(v, d, 64);
-    if ((int)(threadIdx.x & 63) >= d) v += o;
-  }
-  return v;
 }
 
 // One group's span (all waves, any lane).
