@@ -18,7 +18,7 @@ struct WgradArgs {
 // The stages of A go round D buffers, those of B round D + 1: while a stage is multiplied, the next of A and
 // the next two of B are on their way (D = 2; five buffers are what the LDS holds of 256 x 256 tiles, and a load takes
 // longer than a stage).  B are the weights, which come from memory, each group's own, where rows come from L2
-// for all but one of their column tiles (32 groups of about 512 x 2048 x 2048: XXX us, with the third buffer A's YYY).
+// for all but one of their column tiles (8192^3: 851 us, with the third buffer A's 874; its input gradient 870, 906).
 // One barrier per stage; the loads are issued between the matrix instructions of its first half, since a burst
 // of them behind the barrier holds up every wave of the workgroup.
 // KG > 1: KG groups of WM x WN waves share the tile, group g taking the stages g, g + KG, ..
@@ -185,8 +185,16 @@ template <int ES, int WM, int WN, int MT, int NT, int KG, int D, bool VEC>
 __global__ __launch_bounds__(WM * WN * KG * 64, 2) void grouped_wgrad_kernel(WgradArgs a) {
   typedef Core<ES, true, true, WM, WN, MT, NT, KG, D, VEC> C;
   __shared__ __attribute__((aligned(1024))) char smem[KG * C::RING];
-  const int tiles = a.ntiles * a.ktiles;
-  const int e = blockIdx.x / (tiles * a.splits), at = blockIdx.x % (tiles * a.splits);
+  // Workgroups go round the 8 XCDs: of every 256 tiles XCD x takes the x-th eighth, so that a group's rows come through
+  // the L2 of an XCD or two instead of all eight, and every XCD meets long groups and short ones (32 groups of
+  // about 512 x 2048 x 2048: 248 us; tiles in their order 252, 576 MB fetched of 134; an eighth of all tiles 271.  One
+  // group of 16384 x 2048 x 2048: 141 us, in their order 165).
+  const int tiles = a.ntiles * a.ktiles, total = tiles * a.splits * a.groups;
+  const int xcd = blockIdx.x & 7, window = blockIdx.x >> 8 << 8, at_xcd = blockIdx.x >> 3 & 31;
+  const int here = min(256, total - window), share = (here + 7) >> 3;
+  if (at_xcd >= share || xcd * share + at_xcd >= here) return;
+  const int idx = window + xcd * share + at_xcd;
+  const int e = idx / (tiles * a.splits), at = idx % (tiles * a.splits);
   const int split = at / tiles, nt = at % tiles / a.ktiles, kt = at % a.ktiles;
   const Span g = group_span(a.offsets, a.groups, a.rows, e);
   const int group = KG == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / C::NTH), tid = threadIdx.x - group * C::NTH;
@@ -381,7 +389,7 @@ int launch_wgrad(WgradArgs a, hipStream_t stream) {
   a.ktiles = (a.k + WN * NT * 32 - 1) / (WN * NT * 32);
   const long long grid = (long long)a.groups * a.ntiles * a.ktiles * a.splits;
   if (grid >= (1ll << 30)) return C2D_ERR_UNSUPPORTED;
-  hipLaunchKernelGGL((grouped_wgrad_kernel<ES, WM, WN, MT, NT, KG, D, VEC>), dim3((unsigned)grid), dim3(WM * WN * KG * 64), 0, stream, a);
+  hipLaunchKernelGGL((grouped_wgrad_kernel<ES, WM, WN, MT, NT, KG, D, VEC>), dim3((unsigned)((grid + 255) / 256 * 256)), dim3(WM * WN * KG * 64), 0, stream, a);
   return c2d_launch_status();
 }
 
