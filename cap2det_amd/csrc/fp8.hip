@@ -478,13 +478,12 @@ int launch_fp8(const FewArgs& a, hipStream_t stream) {
     const double rows = a.offsets ? (double)a.rows / side + 0.4 * groups : (double)((a.rows + side - 1) / side);
     return rows * ((a.n + side - 1) / side);
   };
-  auto rounds = [](double t, double slots) { return t <= slots ? 1.0 : t / slots; };
   const double kb = a.kb, wide = OUT16 ? 1.0 : 1.5;
-  const double t128 = tiles(128);
-  const double us256 = rounds(tiles(256), 256) * (1.95 * kb + 3.5);
-  const double us128 = t128 <= 256 ? 0.75 * wide * kb + 3.5 : rounds(t128, 512) * (1.3 * wide * kb + 3.5);
-  const double us64 = rounds(tiles(64), 256) * (0.28 * wide * kb + 3.5);
-  const double us32 = rounds(tiles(32), 256) * 0.29 * kb + 2.5;
+  const double t256 = tiles(256), t128 = tiles(128);
+  const double us256 = rounds_of(t256, 256, true) * ((t256 <= 256 ? 1.5 : 1.95) * kb + 3.5);
+  const double us128 = rounds_of(t128, 512, true) * ((t128 <= 256 ? 0.75 : 1.3) * wide * kb + 3.5);
+  const double us64 = rounds_of(tiles(64), 256, false) * (0.28 * wide * kb + 3.5);
+  const double us32 = tiles(32) / 256 * 0.29 * kb + 2.5;
   if (OUT16 && VEC && us256 <= us128 && us256 <= us64 && us256 <= us32)
     return launch_tiles<E5M2, 4, 2, 2, 4, 1, 2, true, true>(a, stream);
   if (us128 <= us64 && us128 <= us32) return launch_tiles<E5M2, 2, 2, 2, 2, 1, 2, VEC, OUT16>(a, stream);

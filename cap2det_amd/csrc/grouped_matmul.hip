@@ -259,8 +259,6 @@ __global__ __launch_bounds__(256) void join_shares_kernel(const float* __restric
 // Up to 16 rows a group, forward: 16 x 16 from registers.  fp32 is bound by its matrix instructions (a stage of a
 // 64 x 64 tile 0.56, of 128 x 128 1.9 or, two per CU, 3.8) and has no 256 x 256 tiles, which gain 2.5 % on
 // 4096^3 and lose wherever tiles are few (4 groups of 1024 x 416 x 1024: 241 against 42 in 64 x 64 tiles).
-double rounds_of(double tiles, double slots) { return tiles <= slots ? 1.0 : tiles / slots; }
-
 enum Shape { T256, T128, T64, T32, T16 };
 Shape rows_shape(const FewArgs& a, int es, bool forward, bool vec) {
   const int groups = a.groups < a.rows ? a.groups : a.rows;
@@ -268,12 +266,12 @@ Shape rows_shape(const FewArgs& a, int es, bool forward, bool vec) {
   auto tiles = [&](int side) { return ((double)a.rows / side + 0.4 * groups) * ((a.n + side - 1) / side); };
   const double stages = ((long long)a.k * es + 127) / 128;
   const double t256 = tiles(256), t128 = tiles(128);
-  const double us256 = t256 <= 256 ? (forward ? 1.2 : 1.5) * stages + 3.5 : rounds_of(t256, 256) * (1.65 * stages + 3.5);
+  const double us256 = t256 <= 256 ? (forward ? 1.2 : 1.5) * stages + 3.5 : rounds_of(t256, 256, true) * (1.65 * stages + 3.5);
   // (128 x 128: from one workgroup per CU to two)
   const double one = es == 4 ? 1.9 : 0.55, two = es == 4 ? 3.8 : forward ? 1.0 : 1.55;
-  const double us128 = rounds_of(t128, 512) * ((t128 <= 256 ? one : t128 >= 512 ? two : one + (two - one) * (t128 - 256) / 256) * stages + 3.5);
-  const double us64 = rounds_of(tiles(64), 256) * ((es == 4 ? 0.56 : 0.25) * stages + 3.0);
-  const double us32 = forward ? rounds_of(tiles(32), 256) * (es == 4 ? 0.4 : 0.29) * stages + 2.5 : 1e30;
+  const double us128 = rounds_of(t128, 512, true) * ((t128 <= 256 ? one : t128 >= 512 ? two : one + (two - one) * (t128 - 256) / 256) * stages + 3.5);
+  const double us64 = rounds_of(tiles(64), 256, false) * ((es == 4 ? 0.56 : 0.25) * stages + 3.0);
+  const double us32 = forward ? tiles(32) / 256 * (es == 4 ? 0.4 : 0.29) * stages + 2.5 : 1e30;
   if (es == 2 && vec && us256 <= us128 && us256 <= us64 && us256 <= us32) return T256;
   if (us128 <= us64 && us128 <= us32) return T128;
   return us64 <= us32 ? T64 : T32;
@@ -291,9 +289,9 @@ WgradPlan wgrad_plan(int groups, int rows, int n, int k, int es) {
     const double slots = side == 128 ? 512 : 256;
     const double stage = es == 4 ? (side == 128 ? 3.8 : 0.56) : side == 256 ? 1.7 : side == 128 ? 1.2 : 0.27;
     const double round = side == 256 ? 20 : side == 128 ? 11 : 4;
-    for (int splits = 1; splits <= 32 && 4 * splits <= stages + 3 && (splits == 1 || splits * mb <= 256); splits *= 2) {
+    for (int splits = 1; splits == 1 || (splits <= 32 && 4 * splits <= stages && splits * mb <= 256); splits *= 2) {
       const double one = side == 128 && tiles * splits <= 256 ? 0.6 : 1.0;  // (one workgroup per CU)
-      const double t = rounds_of(tiles * splits, slots) * one * (stage * stages / splits + round) +
+      const double t = rounds_of(tiles * splits, slots, false) * one * (stage * stages / splits + round) +
                        (splits > 1 ? 4.0 + (splits + 1) * mb / 4.0 : 0.0);
       if (t < least) { least = t; best = {side, splits}; }
     }

@@ -444,6 +444,14 @@ struct Store {
   }
 };
 
+// Rounds in which `slots` resident workgroups make that many tiles.  The last one, where it is half empty or more, is made
+// of halves (place_tile).
+inline double rounds_of(double tiles, double slots, bool halves) {
+  if (tiles <= slots) return 1.0;
+  const double whole = (double)(long long)(tiles / slots), rest = tiles / slots - whole;
+  return whole + (rest < 0.02 ? 0.0 : halves && rest <= 0.5 ? 0.7 : 1.0);
+}
+
 // Workgroups with this much LDS that an XCD of this process holds at a time.
 inline int slots_per_xcd(int lds_bytes) {
   const int n = c2d_available_cus() / 8 * (160 * 1024 / lds_bytes);
