@@ -5,6 +5,7 @@ the hand-written HIP kernels behind these calls.  No fallback: a missing library
 """
 import ctypes
 import functools
+import threading
 
 import torch
 
@@ -844,7 +845,8 @@ def x9_planes(t):
 #
 # Matrices may be row-strided views (columns contiguous).  Everything is queued on the current stream of the
 # current device, where the tensors have to be; results and workspaces of one call are the call's own, so
-# that calls on several streams and captured graphs share none.  A step plan holds addresses: hand it `out`.
+# that calls on several streams and graphs captured into memory pools of their own share none.  A step plan
+# keeps those of the calls that it recorded, since it holds their addresses.
 
 FP8_BLOCK = 128
 FP8_TYPES = (torch.float8_e4m3fn, torch.float8_e5m2)
@@ -855,6 +857,13 @@ _PRODUCT_TYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float8_e4m3fn: 2, to
 def _device():
   """The current device's number (the private query that _stream uses costs a tenth of the public one)."""
   return torch.cuda.current_device() if _cur_device is None else _cur_device()
+
+
+def _own(t):
+  """A result or workspace that a call allocated; a step plan that records the call keeps it."""
+  if _lib.recorder is not None and threading.get_ident() == _lib.recorder_thread:
+    _lib.recorder.keep.append(t)
+  return t
 
 
 def _names(types):
@@ -956,8 +965,8 @@ def fp8_quantize(x, block_rows=1, dtype=torch.float8_e4m3fn):
     batch, step = shape[0], x.stride(0)
     ld = _pitch(x[0], "x") if batch else cols
     grid = (batch,) + grid
-  q = x.new_empty(shape, dtype=dtype)
-  scale = x.new_empty(grid, dtype=_F32)
+  q = _own(x.new_empty(shape, dtype=dtype))
+  scale = _own(x.new_empty(grid, dtype=_F32))
   if batch and rows and cols:
     _lib.call("c2dp_fp8_quantize", x.data_ptr(), _PRODUCT_TYPE[x.dtype], ld, step, q.data_ptr(), _PRODUCT_TYPE[dtype],
               scale.data_ptr(), batch, rows, cols, block_rows, _stream())
@@ -989,7 +998,7 @@ def _fp8_product(a, a_scale, b, b_scale, offsets, groups, rows, n, k, out, out_d
   if out is None:
     if out_dtype is not _BF16 and out_dtype is not _F32:
       raise ValueError("out_dtype: one of %s is wanted, got %s" % (_names(_WIDE_TYPES), out_dtype))
-    y, ldy, clear = a.new_empty((rows, n), dtype=out_dtype), n, 1
+    y, ldy, clear = _own(a.new_empty((rows, n), dtype=out_dtype)), n, 1
   else:
     y, clear = out, 0
     _given_result(y, (rows, n), _WIDE_TYPES, _device(), (a, a_scale, b, b_scale, bias, offsets))
@@ -1060,9 +1069,9 @@ def _grouped_rows(entry, x, name, w, offsets, out, out_dtype, dgrad):
   rows, wide = x.shape[0], k if dgrad else n
   if out is None:
     if out_dtype is None or out_dtype is x.dtype:
-      y = x.new_empty((rows, wide))
+      y = _own(x.new_empty((rows, wide)))
     elif out_dtype is _F32:
-      y = x.new_empty((rows, wide), dtype=_F32)
+      y = _own(x.new_empty((rows, wide), dtype=_F32))
     else:
       raise ValueError("out_dtype: %s or %s for operands of %s, got %s" % (_F32, x.dtype, x.dtype, out_dtype))
     ldy, clear = wide, 1
@@ -1112,14 +1121,14 @@ def grouped_matmul_wgrad(x, dy, offsets, out=None, accumulate=False):
   if out is None:
     if accumulate:
       raise ValueError("accumulate: there is no `out` to add to")
-    dw = x.new_empty((groups, n, k), dtype=_F32)
+    dw = _own(x.new_empty((groups, n, k), dtype=_F32))
   else:
     dw = out
     _whole(dw, "out", (_F32,), (groups, n, k), _device())
     _given_result(dw, (groups, n, k), (_F32,), _device(), (x, dy, offsets))
   if n and k:
     nbytes = _wgrad_workspace_bytes(groups, rows, n, k, _PRODUCT_TYPE[x.dtype])
-    ws = x.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+    ws = _own(x.new_empty(nbytes, dtype=torch.uint8)) if nbytes else None
     _lib.call("c2dp_grouped_matmul_wgrad", x.data_ptr(), _PRODUCT_TYPE[x.dtype], _pitch(x, "x"), dy.data_ptr(),
               _pitch(dy, "dy"), offsets.data_ptr(), groups, dw.data_ptr(), rows, n, k, 1 if accumulate else 0,
               None if ws is None else ws.data_ptr(), nbytes, _stream())

@@ -158,6 +158,29 @@ def test_a_step_plan_replays_the_products_on_other_tensors():
       assert torch.equal(got, want)
 
 
+def test_a_step_plan_keeps_its_workspaces_and_results():
+  """Replays write into memory that nobody else has been given since the recording."""
+  from cap2det_amd.step_plan import StepPlan
+  gen = _gen(26)
+  offs = _offs([0, 8192])
+  x, dy = torch.randn(8192, 256, generator=gen, device="cuda").to(BF16), torch.randn(8192, 192, generator=gen, device="cuda").to(BF16)
+  out, w = torch.empty(1, 192, 256, device="cuda"), torch.randn(1, 192, 256, generator=gen, device="cuda").to(BF16)
+  want, y = ops.grouped_matmul_wgrad(x, dy, offs), ops.grouped_matmul(x, w, offs)
+  plan = StepPlan()
+  with plan.recording():
+    ops.grouped_matmul_wgrad(x, dy, offs, out=out)
+    ops.grouped_matmul(x, w, offs)
+    ops.fp8_quantize(x)
+  torch.cuda.synchronize()
+  others = [torch.full((1 << e,), 7, dtype=torch.uint8, device="cuda") for e in range(12, 25) for _ in range(4)]
+  for _ in range(3):
+    out.fill_(NAN)
+    plan.replay({}, {})
+    torch.cuda.synchronize()
+    assert torch.equal(out, want) and all(bool((t == 7).all()) for t in others)
+  assert any(t.shape == y.shape and torch.equal(t, y) for t in plan.keep)
+
+
 @pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("counts,n,k", [([100, 0, 37], 200, 328), ([9, 3, 1, 0], 96, 640)])
 def test_real_values_within_the_rounding_of_sums(dtype, counts, n, k):

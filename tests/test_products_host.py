@@ -4,6 +4,7 @@ import ctypes
 import os
 import re
 import subprocess
+import threading
 
 import pytest
 import torch
@@ -187,6 +188,39 @@ def test_calls_that_are_accepted_and_what_they_pass_on(calls):
   ops.grouped_matmul(x[:0], w, OFFS)
   ops.fp8_quantize(_t(0, 7))
   assert not calls
+
+
+def test_a_step_plan_keeps_what_the_calls_that_it_records_allocate(calls, monkeypatch):
+  class Recorder(object):
+    keep = []
+  monkeypatch.setattr(_lib, "recorder", Recorder)
+  x, dy = _t(8192, 256, dtype=BF16), _t(8192, 192, dtype=BF16)
+  offs = torch.tensor([0, 8192], dtype=torch.int32)
+  v, w = _fp8_args(), _t(1, 192, 256, dtype=BF16)
+
+  def run():
+    """Addresses that the calls write to."""
+    ops.grouped_matmul_wgrad(x, dy, offs, out=torch.zeros(1, 192, 256))
+    held = {calls[-1][-3]}
+    ops.grouped_matmul_wgrad(x, dy, offs)
+    held |= {calls[-1][8], calls[-1][-3]}
+    ops.fp8_quantize(x)
+    held |= {calls[-1][5], calls[-1][7]}
+    ops.fp8_matmul(**v)
+    held.add(calls[-1][11])
+    for dtype in (BF16, F32):
+      ops.grouped_matmul(x, w, offs, out_dtype=dtype)
+      held.add(calls[-1][7])
+    assert None not in held
+    return held
+
+  monkeypatch.setattr(_lib, "recorder_thread", threading.get_ident())
+  assert run() == {t.data_ptr() for t in Recorder.keep}
+  kept = len(Recorder.keep)
+  monkeypatch.setattr(_lib, "recorder_thread", -1)                 # (another thread records)
+  run()
+  assert len(Recorder.keep) == kept
+  calls.clear()
 
 
 X, W, DY = _t(4, 24, dtype=BF16), _t(2, 16, 24, dtype=BF16), _t(4, 16, dtype=BF16)
