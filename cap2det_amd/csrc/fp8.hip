@@ -325,11 +325,10 @@ __device__ __forceinline__ void fp8_tile(const FewArgs& a, const Place& p, char*
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
   const int rounds = (a.kb + KG - 1) / KG;
-  float row_scale[MT], col_scale = 0.0f;
-  // (a stage behind the last is zeros that nobody reads, or that count nothing: its scale is zero)
+  float row_scale[MT], col_scale;
   auto load_scales = [&](int st) {
     const int c = min(st, a.kb - 1);
-    col_scale = st < a.kb ? bs[c] : 0.0f;
+    col_scale = bs[c];
 #pragma unroll
     for (int i = 0; i < MT; ++i) row_scale[i] = as[as_at[i] + (unsigned)c];
   };
@@ -348,7 +347,8 @@ __device__ __forceinline__ void fp8_tile(const FewArgs& a, const Place& p, char*
     stage_barrier<VEC, TB::LOADS + (D - 2) * PASSES>();
     float scale[MT];
 #pragma unroll
-    for (int i = 0; i < MT; ++i) scale[i] = KG > 1 && col_scale == 0.0f ? 0.0f : row_scale[i] * col_scale;
+    for (int i = 0; i < MT; ++i)  // (a group's stage behind the last is zeros, which no scale may make a NaN)
+      scale[i] = KG > 1 && it * KG + group >= a.kb ? 0.0f : row_scale[i] * col_scale;
     load_scales((it + 1) * KG + group);  // in front of the loads to LDS
     const int st_a = (it + DA - 1) * KG + group, st_b = (it + DB - 1) * KG + group;
     const typename TA::Stage ga = ta.at(st_a);

@@ -249,6 +249,23 @@ def test_pitches_garbage_beside_columns_and_bad_values():
   assert got[:, 130].isnan().all() and torch.equal(got[:, :130], want[:, :130].clamp(min=0).float())
 
 
+@pytest.mark.parametrize("out_dtype", [BF16, F32])
+@pytest.mark.parametrize("m,n,k", [(9, 200, 272), (130, 200, 400), (1000, 1000, 1100), (1900, 1900, 272), (4000, 4096, 272)])
+def test_zero_and_infinite_scales(m, n, k, out_dtype):
+  """0 * infinity is a NaN in every kernel; the scales of other rows and columns have no part in it."""
+  gen = _gen(m)
+  a, a_s, b, b_s = _operands(gen, m, n, k, E4M3)
+  a_s[5, 1] = a_s[8, -1] = INF
+  b_s[0, 1] = 0.0
+  got = ops.fp8_matmul(a, a_s, b, b_s, out_dtype=out_dtype)
+  assert got[5, :128].isnan().all() and not got[5].isfinite().any() and not got[8].isfinite().any()
+  a_s[5, 1] = a_s[8, -1] = 0.0
+  want = _want(a, a_s, b, b_s).to(out_dtype)
+  keep = torch.ones(m, dtype=torch.bool, device="cuda")
+  keep[5] = keep[8] = False
+  assert torch.equal(got[keep], want[keep])
+
+
 @pytest.mark.parametrize("m,n,k", [(0, 5, 16), (5, 0, 16), (5, 7, 0)])
 def test_empty_sizes(m, n, k):
   a, b = torch.ones(m, k, device="cuda").to(E4M3), torch.ones(n, k, device="cuda").to(E4M3)
