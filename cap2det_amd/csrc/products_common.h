@@ -458,6 +458,10 @@ inline int slots_per_xcd(int lds_bytes) {
   return n > 0 ? n : 1;
 }
 
+inline bool sizes_fit(int a, int b, int c, int d) {
+  return a <= C2DP_MAX_SIZE && b <= C2DP_MAX_SIZE && c <= C2DP_MAX_SIZE && d <= C2DP_MAX_SIZE;
+}
+
 inline bool aligned16(const void* p, long long pitch_bytes) {
   return ((unsigned long long)p & 15) == 0 && (pitch_bytes & 15) == 0;
 }

@@ -851,6 +851,7 @@ def x9_planes(t):
 FP8_BLOCK = 128
 FP8_TYPES = (torch.float8_e4m3fn, torch.float8_e5m2)
 _WIDE_TYPES = (torch.float32, torch.bfloat16)
+_MAX_SIZE = 1 << 30
 _PRODUCT_TYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float8_e4m3fn: 2, torch.float8_e5m2: 3}
 
 
@@ -880,6 +881,11 @@ def _operand(t, name, types, dims, device):
     raise ValueError("%s: one of %s is wanted, got %s" % (name, _names(types), t.dtype))
   if t.dim() != dims:
     raise ValueError("%s: %d dimensions are wanted, got shape %s" % (name, dims, tuple(t.shape)))
+
+
+def _check_sizes(*sizes):
+  if max(sizes) > _MAX_SIZE:
+    raise ValueError("rows, columns and groups up to %d, got %d" % (_MAX_SIZE, max(sizes)))
 
 
 def _whole(t, name, types, shape, device):
@@ -958,6 +964,7 @@ def fp8_quantize(x, block_rows=1, dtype=torch.float8_e4m3fn):
     raise ValueError("block_rows: 1 or %d, got %r" % (FP8_BLOCK, block_rows))
   shape = x.shape
   rows, cols = shape[-2], shape[-1]
+  _check_sizes(*shape)
   grid = (-(-rows // block_rows), -(-cols // FP8_BLOCK))
   if len(shape) == 2:
     batch, step, ld = 1, 0, _pitch(x, "x")
@@ -995,6 +1002,7 @@ def _check_fp8(a, a_scale, b, b_scale, offsets, bias, dense):
 
 
 def _fp8_product(a, a_scale, b, b_scale, offsets, groups, rows, n, k, out, out_dtype, bias, relu):
+  _check_sizes(groups, rows, n, k)
   if out is None:
     if out_dtype is not _BF16 and out_dtype is not _F32:
       raise ValueError("out_dtype: one of %s is wanted, got %s" % (_names(_WIDE_TYPES), out_dtype))
@@ -1067,6 +1075,7 @@ def _grouped_rows(entry, x, name, w, offsets, out, out_dtype, dgrad):
     _check_grouped(x, name, w, offsets, dgrad)
   groups, n, k = w.shape
   rows, wide = x.shape[0], k if dgrad else n
+  _check_sizes(groups, rows, n, k)
   if out is None:
     if out_dtype is None or out_dtype is x.dtype:
       y = _own(x.new_empty((rows, wide)))
@@ -1118,6 +1127,7 @@ def grouped_matmul_wgrad(x, dy, offsets, out=None, accumulate=False):
     _check_wgrad(x, dy, offsets)
   rows, k = x.shape
   n, groups = dy.shape[1], offsets.shape[0] - 1
+  _check_sizes(groups, rows, n, k)
   if out is None:
     if accumulate:
       raise ValueError("accumulate: there is no `out` to add to")

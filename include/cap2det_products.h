@@ -10,6 +10,7 @@
  *   - a pitch is at most C2DP_MAX_PITCH bytes, else C2D_ERR_UNSUPPORTED.  16-byte aligned base
  *     pointers, pitches and contraction lengths take the direct global -> LDS loads; any others are
  *     right too, through registers, and slower.
+ *   - rows, n, k, cols, batch and groups are at most C2DP_MAX_SIZE, else C2D_ERR_UNSUPPORTED.
  *   - sums are fp32.
  *
  * Groups.  `offsets` is a DEVICE array of groups + 1 int32 row numbers: group e owns the rows
@@ -38,6 +39,7 @@ int c2dp_version(void);
 
 #define C2DP_BLOCK 128             /* elements of the contraction that share a scale */
 #define C2DP_MAX_PITCH (1 << 22)   /* bytes */
+#define C2DP_MAX_SIZE (1 << 30)
 
 /* 8-bit values and fp32 scales of `batch` matrices x [rows][cols] (x_type C2DP_F32 or C2DP_BF16; matrix
  * i begins at x + i * x_batch elements).  Blocks are block_rows x 128, block_rows 1 or 128:

@@ -110,6 +110,23 @@ def test_unsupported_pitches_and_short_workspaces_end_on_the_host():
   assert _wgrad(groups=1, rows=8192, workspace=ODD, workspace_bytes=need) == -1
 
 
+def test_sizes_that_pass_the_limit_end_on_the_host(calls):
+  over = 2 ** 30 + 1
+  assert _fp8(rows=over) == -2 and _fp8(n=over, ldy=over) == -2 and _quantize(rows=over) == -2 and _quantize(batch=over) == -2
+  assert _rows(rows=over) == -2 and _rows(groups=over) == -2 and _rows(dgrad=True, rows=over) == -2
+  assert _wgrad(rows=over) == -2 and _wgrad(groups=over) == -2
+  for many in (over, 2 ** 32 + 5):                           # (as 32-bit numbers the latter would be 5 rows)
+    x, one = _t(1, 24, dtype=BF16).expand(many, 24), torch.zeros(2, dtype=torch.int32)
+    a, s = torch.empty(many, 0, dtype=E4M3), torch.empty(many, 0)
+    for f in (lambda: ops.fp8_quantize(x), lambda: ops.fp8_matmul(a, s, _t(8, 0, dtype=E4M3), _t(1, 0)),
+              lambda: ops.grouped_matmul_fp8(a, s, _t(1, 8, 0, dtype=E4M3), _t(1, 1, 0), one),
+              lambda: ops.grouped_matmul(x, W[:1], one), lambda: ops.grouped_matmul_dgrad(x, _t(1, 24, 8, dtype=BF16), one),
+              lambda: ops.grouped_matmul_wgrad(x, x, one)):
+      with pytest.raises(ValueError, match="rows, columns and groups up to 1073741824"):
+        f()
+  assert not calls
+
+
 def test_empty_calls_are_no_calls():
   for empty in (dict(rows=0), dict(cols=0, ldx=0), dict(batch=0)):
     assert _quantize(x=None, q=None, scale=None, **empty) == 0
