@@ -388,6 +388,13 @@ __device__ __forceinline__ unsigned pack_bf16(float a, float b) {
 template <class V>
 __device__ __forceinline__ void store_at(char* p, V v) { __builtin_memcpy(p, &v, sizeof(V)); }
 
+// LDS writes of a wave's lanes before it, reads of others after it (they happen in the program's order: this holds the
+// compiler to it).
+__device__ __forceinline__ void lanes_in_order() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
 // A wave's MT x NT result tiles of 32 x 32: lane l holds row m = l & 31, register r column 8 (r >> 2) + 4 (l >> 5) +
 // (r & 3).  They go to memory through LDS, 32 rows at a time, so that a store writes whole rows of the wave's
 // columns, 16 bytes a lane: straight from the registers an instruction would write 32 bytes of each of 32
@@ -417,6 +424,7 @@ struct Store {
           if constexpr (BF16) *(u32x2*)to = u32x2{pack_bf16(v[4 * g], v[4 * g + 1]), pack_bf16(v[4 * g + 2], v[4 * g + 3])};
           else *(f32x4*)to = f32x4{v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]};
         }
+      lanes_in_order();
 #pragma unroll
       for (int t = 0; t < 32 / STEP; ++t) {
         const int r = t * STEP + lane / LANES, m = i * 32 + r;
@@ -440,6 +448,7 @@ struct Store {
           }
         }
       }
+      lanes_in_order();
     }
   }
 };
