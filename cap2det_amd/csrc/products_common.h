@@ -298,8 +298,11 @@ struct Tile {
 #ifdef __HIP_DEVICE_COMPILE__  // (the host pass refuses 16 bytes here, and with that drops some kernels' stubs)
       const int soff = __builtin_amdgcn_readfirstlane(g.k0 + i * RPP * (int)ld);
       char* const lds = to + i * NTH * 16 + wave * 1024;
-      if constexpr (UNSEEN) {  // (the low half of an LDS pointer is its offset)
-        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+      if constexpr (UNSEEN) {
+        // The low half of an LDS pointer is its offset.  A scalar register that a vector instruction wrote (readfirstlane)
+        // may be read by a load five wait states later, which the compiler sees to for loads that it knows: s_mov's
+        // one and s_nop's five.
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
                      :: "s"(__builtin_amdgcn_readfirstlane((int)(unsigned long long)lds)), "v"(g.off),
                         "s"(buffer_words(g.base, g.bytes)), "s"(soff) : "memory", "m0");
       } else {

@@ -144,6 +144,28 @@ def test_workspace_is_nothing_where_tiles_are_many_or_arguments_are_none():
       assert f(1, rows, 512, 512, kind) <= 256 << 20
 
 
+def test_loads_written_as_assembly_wait_for_their_scalar_operands():
+  """Five wait states lie between a vector instruction's write of a scalar register and a load's read of it; the compiler
+  counts none for a load inside inline assembly, so the block has them: one an instruction, n + 1 of s_nop n."""
+  csrc = os.path.join(os.path.dirname(_lib.__file__), "csrc")
+  found = 0
+  for name in sorted(os.listdir(csrc)):
+    if name.endswith((".h", ".hip")):
+      with open(os.path.join(csrc, name)) as f:
+        blocks = re.findall(r'asm volatile\(((?:\s*"[^"]*")+)', f.read())
+      for block in blocks:
+        waited = 0
+        for line in "".join(re.findall(r'"([^"]*)"', block)).replace("\\t", "").split("\\n"):
+          op = line.split()
+          if not op:                                         # (a barrier for the compiler alone)
+            continue
+          if op[0].startswith(("buffer_load", "buffer_store", "global_load", "global_store")):
+            found += 1
+            assert waited >= 5, (name, block)
+          waited += int(op[1]) + 1 if op[0] == "s_nop" else 1
+  assert found
+
+
 # -- wrappers -------------------------------------------------------------------------------------
 
 @pytest.fixture
