@@ -187,8 +187,8 @@ __global__ __launch_bounds__(WM * WN * KG * 64, 2) void grouped_wgrad_kernel(Wgr
   __shared__ __attribute__((aligned(1024))) char smem[KG * C::RING];
   // Workgroups go round the 8 XCDs: of every 256 tiles XCD x takes the x-th eighth, so that a group's rows come through
   // the L2 of an XCD or two instead of all eight, and every XCD meets long groups and short ones (32 groups of
-  // about 512 x 2048 x 2048: 248 us; tiles in their order 252, 576 MB fetched of 134; an eighth of all tiles 271.  One
-  // group of 16384 x 2048 x 2048: 141 us, in their order 165).
+  // about 512 x 2048 x 2048: 242 us; tiles in their order 252, 576 MB fetched of 134; an eighth of all tiles 271.  One
+  // group of 16384 x 2048 x 2048: 138 us, in their order 165).
   const int tiles = a.ntiles * a.ktiles, total = tiles * a.splits * a.groups;
   const int xcd = blockIdx.x & 7, window = blockIdx.x >> 8 << 8, at_xcd = blockIdx.x >> 3 & 31;
   const int here = min(256, total - window), share = (here + 7) >> 3;

@@ -301,8 +301,8 @@ struct Tile {
       if constexpr (UNSEEN) {
         // The low half of an LDS pointer is its offset.  A scalar register that a vector instruction wrote (readfirstlane)
         // may be read by a load five wait states later, which the compiler sees to for loads that it knows: s_mov's
-        // one and s_nop's five.
-        asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+        // one and s_nop's four (input gradient of 8 groups of 512 x 1024 x 1024: 18.7 us, without them 18.2).
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
                      :: "s"(__builtin_amdgcn_readfirstlane((int)(unsigned long long)lds)), "v"(g.off),
                         "s"(buffer_words(g.base, g.bytes)), "s"(soff) : "memory", "m0");
       } else {

@@ -53,7 +53,7 @@ int c2dp_fp8_quantize(const void* x, int x_type, long long ldx, long long x_batc
 
 /* y[i][j] = act( sum over blocks c of 128 k of
  *                  a_scale[i][c] * b_scale[e][j / 128][c] * sum_{k in c} a[i][k] * b[e][j][k]
- *                + bias[e][j] ),   e the group of row i.
+ *                + bias[e][j] ),   e the group of row i; the two scales are multiplied first, as fp32.
  *   a       [rows][k]       C2DP_E4M3 or C2DP_E5M2 (a_type), pitch lda
  *   a_scale [rows][ceil(k / 128)]
  *   b       [groups][n][k]  C2DP_E4M3, contiguous
