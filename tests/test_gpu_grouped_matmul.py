@@ -73,10 +73,11 @@ def test_larger_products_of_integers_are_exact(dtype, counts, n, k):
   _same(ops.grouped_matmul_wgrad(x, dy, offs), up.grouped_dw(x, dy, offsets))
 
 
-# Sizes at which the estimated times choose 256 x 256 tiles, with groups whose last tile is short, long and whole, more
+# Sizes at which the estimated times choose 256 x 256 and (last) 128 x 256 tiles, with groups whose last tile is short, long and whole, more
 # row tiles than an XCD holds at a time, and (5800 rows of 2048 columns) a last round that is made as halves
 @pytest.mark.parametrize("counts,n,k", [([3000, 100, 5900], 2048, 1024), ([5800], 2048, 1024), ([600, 0, 130, 256, 2000, 385] * 2, 1100, 1032),
-                                        ([37 * i % 299 for i in range(150)], 520, 1032), ([128] * 65 + [0, 1, 500], 1032, 264)])
+                                        ([37 * i % 299 for i in range(150)], 520, 1032), ([128] * 65 + [0, 1, 500], 1032, 264),
+                                        ([1500, 1000, 1, 1999], 1024, 2048), ([1700, 0, 2592], 1880, 1512), ([4096], 2048, 2048)])
 def test_large_tiles_of_integers_are_exact(counts, n, k):
   gen = _gen(21)
   offsets = up.offsets_of(counts, first=5)
