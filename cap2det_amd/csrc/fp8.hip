@@ -8,10 +8,9 @@ namespace {
 
 // ---- quantiser --------------------------------------------------------------------------------------
 //
-// scale = max(max |x| / F, 2^-126), q = rne8(x / scale).  The quotient is x * r with r = 1 / scale correctly
-// rounded, and one correction by its own remainder (Markstein's theorem: the quotient is then correctly
-// rounded too): three operations an element where a division takes ten, and no value near a tie falls on
-// another side than the true quotient's.  |x| <= F * scale up to rounding, so nothing overflows the type.
+// s = max(max |x| / F, 2^-126), scale = s as fp32, q = rne8(x / s), rounded once: x / scale as fp32 lies on another side of
+// a tie than x / s in about one of a million values, which is then a whole step off.  |x| <= F s, so nothing
+// overflows the type.
 
 // (any address)
 __device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
@@ -53,19 +52,15 @@ __device__ __forceinline__ float largest_of_16_lanes(float m) {
 }
 
 template <bool E5M2>
+constexpr float LARGEST = E5M2 ? 57344.0f : 448.0f;  // F = 7 * 2^i
+
+template <bool E5M2>
 __device__ __forceinline__ float scale_of(float m) {
-  return fmaxf(m / (E5M2 ? 57344.0f : 448.0f), 0x1p-126f);
+  return fmaxf(m / LARGEST<E5M2>, 0x1p-126f);
 }
 
 template <bool E5M2>
-__device__ __forceinline__ u32x2 quantize8(const float (&v)[8], float scale) {
-  const float r = 1.0f / scale;
-  float q[8];
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const float t = v[j] * r;
-    q[j] = fmaf(fmaf(-t, scale, v[j]), r, t);
-  }
+__device__ __forceinline__ u32x2 to_8_bits(const float (&q)[8]) {
   u32x2 o;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
@@ -80,6 +75,54 @@ __device__ __forceinline__ u32x2 quantize8(const float (&v)[8], float scale) {
     o[h] = (unsigned)w;
   }
   return o;
+}
+
+// x / s rounded so that its rounding to 8 bits is that of the true quotient.  The quotient is t + c, t = x r and c its
+// correction: the remainder x - t s, exact (one fused multiply-add), by r, and what the scale's rounding makes (rho).
+// Their sum's own rounding leaves e, known to 2^-44 of the quotient: where there is one, the result is the odd one of
+// the two fp32 numbers around the quotient, which lies on the same side of every tie as the quotient does.
+template <bool E5M2>
+__device__ __forceinline__ void quotients(const float (&v)[8], float m, float scale, float (&q)[8]) {
+#pragma clang fp contract(off)  // (t is the rounded product in all of its uses)
+  const float up = m < 0x1p-40f ? 0x1p80f : 1.0f;  // (no remainder is a denormal number)
+  const float s = scale * up, r = 1.0f / s, top = m * up;
+  const float rho = scale > 0x1p-126f ? fmaf(-s, LARGEST<E5M2>, top) / top : 0.0f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float x = v[j] * up, t = x * r;
+    const float c = fmaf(-t, rho, fmaf(-t, s, x) * r);
+    const float sum = t + c, e = c - (sum - t);
+    int bits = __float_as_int(sum);
+    if (fabsf(e) > 0x1p-40f * fabsf(sum) && !(bits & 1)) bits += (bits ^ __float_as_int(e)) < 0 ? -1 : 1;
+    q[j] = __int_as_float(bits);
+  }
+}
+
+// m: the block's largest |x|.
+// bf16: a quotient is a tie, or 2^-13 of it or more away from one: X and M being whole numbers below 256, 7 X 2^i and
+// T M differ by one or more, T < 32.  x * (1 / s) is within 2^-22 of it: rounded to 21 bits it is on the tie, or on its side.
+// fp32: x by 1 / s made smaller and larger by 2^-21 are on either side of the quotient.  Where both round to the same
+// it does too; where not, in one of some 10^5 random values, the quotient is made with care.
+template <class T, bool E5M2>
+__device__ __forceinline__ u32x2 quantize8(const float (&v)[8], float m, float scale) {
+  const float r = scale < __builtin_inff() ? 1.0f / scale : __builtin_nanf("");  // (an infinity makes NaNs of its block)
+  float q[8];
+  if constexpr (std::is_same<T, __bf16>::value) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) q[j] = __int_as_float((__float_as_int(v[j] * r) + 4) & ~7);
+    return to_8_bits<E5M2>(q);
+  } else {
+    const float below = r * (1.0f - 0x1p-21f), above = r * (1.0f + 0x1p-21f);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) q[j] = v[j] * below;
+    const u32x2 o = to_8_bits<E5M2>(q);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) q[j] = v[j] * above;
+    const u32x2 p = to_8_bits<E5M2>(q);
+    if (o[0] == p[0] && o[1] == p[1]) return o;
+    quotients<E5M2>(v, m, scale, q);
+    return to_8_bits<E5M2>(q);
+  }
 }
 
 __device__ __forceinline__ void store_chunk(unsigned char* row, int c, int cols, u32x2 q) {
@@ -130,9 +173,9 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(QuantArgs a) {
     if (t < tasks) {
       const int r = wide ? 0 : a.kb == 1 ? t : (int)__umulhi((unsigned)t, a.magic);
       const int j = wide ? j0 + t : t - r * a.kb;
-      const float s = scale_of<E5M2>(largest_of_16_lanes(largest(v[u])));
+      const float m = largest_of_16_lanes(largest(v[u])), s = scale_of<E5M2>(m);
       const long long row = (long long)blockIdx.z * a.rows + row0 + r;
-      store_chunk(a.q + row * a.cols, j * 128 + lane16 * 8, a.cols, quantize8<E5M2>(v[u], s));
+      store_chunk(a.q + row * a.cols, j * 128 + lane16 * 8, a.cols, quantize8<T, E5M2>(v[u], m, s));
       if (lane16 == 0) a.scale[row * a.kb + j] = s;
     }
   }
@@ -172,7 +215,7 @@ __global__ __launch_bounds__(2048 / U) void quantize_square_kernel(QuantArgs a) 
   for (int u = 0; u < U; ++u) {
     const int r = bi * 128 + slot + STEP * u;
     if (r < a.rows)
-      store_chunk(a.q + ((long long)blockIdx.y * a.rows + r) * a.cols, c, a.cols, quantize8<E5M2>(v[u], s));
+      store_chunk(a.q + ((long long)blockIdx.y * a.rows + r) * a.cols, c, a.cols, quantize8<T, E5M2>(v[u], m, s));
   }
   if (threadIdx.x == 0) a.scale[((long long)blockIdx.y * mb + bi) * a.kb + bj] = s;
 }

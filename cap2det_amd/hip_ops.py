@@ -953,8 +953,8 @@ def fp8_quantize(x, block_rows=1, dtype=torch.float8_e4m3fn):
   (q [.., rows, cols], scale [.., ceil(rows / block_rows), ceil(cols / 128)]), x ~ q * scale of its block.
 
   Blocks are block_rows x 128: 1 for activations, 128 for weights.  scale = max |x| / F, at least
-  2^-126, F = 448 (float8_e4m3fn) or 57344 (float8_e5m2); q = x / scale in fp32, to the nearest, ties to
-  even.  A NaN stays one and takes no part in the maximum, an infinity makes its block's values NaN.
+  2^-126, F = 448 (float8_e4m3fn) or 57344 (float8_e5m2); q = the value nearest to x / scale, ties to even, rounded
+  once (the scale as it is before its rounding to fp32).  A NaN stays one and takes no part in the maximum, an infinity makes its block's values NaN.
   The blocks of a weight matrix w are square: q.t().contiguous() and scale.t().contiguous() are w.t()'s."""
   if not (isinstance(x, torch.Tensor) and x.get_device() == _device() and x.dtype in _WIDE_TYPES and x.dim() == 2):
     _operand(x, "x", _WIDE_TYPES, 3 if isinstance(x, torch.Tensor) and x.dim() == 3 else 2, _device())

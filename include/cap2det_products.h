@@ -43,9 +43,9 @@ int c2dp_version(void);
 
 /* 8-bit values and fp32 scales of `batch` matrices x [rows][cols] (x_type C2DP_F32 or C2DP_BF16; matrix
  * i begins at x + i * x_batch elements).  Blocks are block_rows x 128, block_rows 1 or 128:
- *   scale = max(max |x| of the block / F, 2^-126),  q = x / scale as fp32, rounded to the nearest, ties to
- * even; F is the largest value of q_type (C2DP_E4M3 / C2DP_E5M2).  A NaN stays one and takes no part in the maximum;
- * an infinity makes every value of its block a NaN.
+ *   s = max(max |x| of the block / F, 2^-126),  scale = s as fp32,  q = the 8-bit value nearest to x / s (s as
+ * it is before it is rounded), ties to even; F is the largest value of q_type (C2DP_E4M3 / C2DP_E5M2).  A NaN stays one
+ * and takes no part in the maximum; an infinity makes every value of its block a NaN.
  *   q     [batch][rows][cols]
  *   scale [batch][ceil(rows / block_rows)][ceil(cols / 128)] */
 int c2dp_fp8_quantize(const void* x, int x_type, long long ldx, long long x_batch, void* q, int q_type,

@@ -20,17 +20,27 @@ def _offs(offsets):
   return torch.tensor(offsets, dtype=torch.int32, device="cuda")
 
 
+def _nearest(v, to):
+  """float64 -> the nearest 8-bit value, ties to even, in one rounding: whole numbers of the value's own step."""
+  bits, least = (3, -6) if to == E4M3 else (2, -14)
+  exponent = (torch.frexp(v.abs())[1] - 1).clamp(min=least).double()
+  step = torch.exp2(exponent - bits)
+  return (torch.round(v / step) * step).float().to(to)
+
+
 def _quantized(x, rows, to):
-  """The definition: both quotients correctly rounded to fp32 (through float64, whose 53 bits are more than twice 24
+  """The definition.  The scale is correctly rounded to fp32 (through float64, whose 53 bits are more than twice 24
   and 2: rounding twice is rounding once; torch divides by a number on the GPU through its reciprocal, which
-  is not), the second then to 8 bits by torch."""
+  is not).  x F is exact in float64, so that its quotient by the largest value is a tie just where the true one is: a tie
+  has at most 5 bits."""
   m, k = x.shape[-2:]
   mb, kb = -(-m // rows), -(-k // 128)
   v = torch.nn.functional.pad(x.float(), (0, kb * 128 - k, 0, mb * rows - m)).view(*x.shape[:-2], mb, rows, kb, 128)
   top = v.abs().nan_to_num(nan=0.0, posinf=INF).amax(dim=(-3, -1))
   scale = (top.double() / MAX[to]).float().clamp(min=2.0 ** -126)
-  q = (v.double() / scale.double()[..., :, None, :, None]).float().reshape(*x.shape[:-2], mb * rows, kb * 128)[..., :m, :k]
-  return q.to(to), scale
+  by = top.double().clamp(min=MAX[to] * 2.0 ** -126)[..., :, None, :, None]
+  q = (v.double() * MAX[to] / by).reshape(*x.shape[:-2], mb * rows, kb * 128)[..., :m, :k]
+  return _nearest(q, to), scale
 
 
 def _bits(t):
@@ -52,6 +62,27 @@ def test_quantize_is_the_definition_bit_for_bit(to, dtype, rows, m, k):
   assert q.dtype == to and q.shape == x.shape and scale.shape == (-(-m // rows), -(-k // 128))
   assert torch.equal(scale, want_s)
   assert torch.equal(_bits(q), _bits(want_q))
+
+
+@pytest.mark.parametrize("to", [E4M3, E5M2])
+@pytest.mark.parametrize("exponent", [-118, -100, -41, -38, 0, 100])
+def test_quantize_rounds_once(to, exponent):
+  """Values one unit in the last place on either side of a tie, and on ties whose scale is not a number of 24 bits (three
+  quarters of the largest value: 21 of the steps), from the least scales to large ones; and millions of random ones."""
+  gen = _gen(exponent + 200)
+  top = (1 + torch.rand(300, 1, generator=gen, device="cuda")) * 2.0 ** exponent
+  ties = (2 * torch.randint(8, 16, (300, 100), generator=gen, device="cuda") + 1) if to == E4M3 else \
+         (2 * torch.randint(4, 8, (300, 100), generator=gen, device="cuda") + 1)
+  x = (top.double() / 1.75 * ties / 16 * torch.exp2(-torch.randint(0, 5, ties.shape, generator=gen, device="cuda").double())).float()
+  x = torch.where(x > top, x / 2, x)
+  bits = x.view(torch.int32) + torch.randint(-1, 2, x.shape, generator=gen, device="cuda").int()
+  even = (top.to(BF16).float() * 0.75) * torch.exp2(-torch.randint(0, 5, (300, 27), generator=gen, device="cuda").float())
+  for v in (torch.cat([bits.view(F32), top, top / 3, -top / 7], 1), torch.cat([even, top.to(BF16).float()], 1),
+            torch.randn(4000, 1000, generator=gen, device="cuda") * 2.0 ** exponent):
+    for rows in (1, 128):
+      q, scale = ops.fp8_quantize(v, rows, to)
+      want_q, want_s = _quantized(v, rows, to)
+      assert torch.equal(scale, want_s) and torch.equal(_bits(q), _bits(want_q))
 
 
 @pytest.mark.parametrize("to", [E4M3, E5M2])
