@@ -12,6 +12,7 @@
 #pragma once
 #include "c2d_common.h"
 #include "../../include/cap2det_products.h"
+#include "products_place.h"
 #include <type_traits>
 
 namespace c2d_pr {
@@ -50,9 +51,6 @@ __device__ __forceinline__ i32x4 buffer_words(const void* p, long long bytes) {
 }
 
 // ---- ragged groups ------------------------------------------------------------------------------
-
-// Group boundaries as they are used: each offset clamped to [0, rows], and at least every earlier one.
-struct Span { int lo, hi; };
 
 // Running sums / maxima (of numbers from 0) over the lanes of a wave: four steps within 16 lanes and two across them, as
 // operands of the vector instructions (DPP).  As shuffles through LDS they were most of a workgroup's start.
@@ -93,31 +91,15 @@ __device__ __forceinline__ Span group_span(const int* __restrict__ offsets, int 
   }
 }
 
-struct Place {
-  int e, lo, hi;   // the tile's group and its rows
-  int m0, nt;      // first row of the tile, column tile
-  bool live;       // false: the workgroup has no tile
-  int begin, end;  // rows outside [begin, end) are in no group
-  int spare, spares;  // a workgroup without a tile: its number among those that clear rows (-1: none)
-};
-
-// Tile of workgroup `bid` out of `nbid` (a multiple of 8).  The host cannot know how many row tiles the
-// groups make; it launches the largest number, rows / BM + groups, and each wave counts them here: one
-// or two loads and two dozen lane shuffles for 64 groups.  Workgroups go round the 8 XCDs by number; XCD x
-// takes the x-th eighth of the tiles, in bands of 4 row tiles by all column tiles, so that what
-// runs there at a time shares rows and weights in that XCD's L2.
-// HALVES: a tile of BM / 2 rows or less costs half, and a group's last one often is.  All of those come behind the
-// others; and where the others end with a round that would leave most of an XCD's `slots` resident
-// workgroups without a tile, the tiles of that round are made as halves too (32 groups of about 512 x 2048 x 2048:
-// 177 us, in the groups' order 180; a half costs 0.7 of a tile, since its loads are three quarters of one's).
+// Tile of workgroup `bid` (products_place.h).  The host cannot know how many row tiles the groups make; it launches the
+// largest number, rows / BM + groups, and each wave counts them here: one or two loads and two dozen lane shuffles
+// for 64 groups.
 template <int BM, bool HALVES>
 __device__ __forceinline__ Place place_tile(const int* __restrict__ offsets, int groups, int rows, int ntiles,
                                             unsigned bid, unsigned nbid, int slots) {
   Place p;
   int carry = 0, full = 0, half = 0;  // row tiles of all groups
   Span s = {0, rows};
-  auto fulls = [](int r) { return HALVES ? (r + BM / 2 - 1) / BM : (r + BM - 1) / BM; };
-  auto halves = [&](int r) { return (r + BM - 1) / BM - fulls(r); };
   int upto_full = 0, upto_half = 0;
   if (!offsets) {
     full = (rows + BM - 1) / BM;
@@ -127,49 +109,20 @@ __device__ __forceinline__ Place place_tile(const int* __restrict__ offsets, int
     for (int base = 0; base < groups; base += 64) {
       s = lane_span(offsets, groups, rows, base, &carry);
       if (base == 0) p.begin = __builtin_amdgcn_readlane(s.lo, 0);
-      upto_full = lane_prefix_sum(fulls(s.hi - s.lo));
+      upto_full = lane_prefix_sum(full_tiles_of<BM, HALVES>(s.hi - s.lo));
       full += __builtin_amdgcn_readlane(upto_full, 63);
       if (HALVES) {
-        upto_half = lane_prefix_sum(halves(s.hi - s.lo));
+        upto_half = lane_prefix_sum(half_tiles_of<BM, HALVES>(s.hi - s.lo));
         half += __builtin_amdgcn_readlane(upto_half, 63);
       }
     }
     p.end = carry;
   }
-  const int xcd = bid & 7, local = bid >> 3, per = nbid >> 3;
-  const int full_tiles = full * ntiles, half_tiles = half * ntiles;
-  const int my_full = (full_tiles + 7 - xcd) >> 3, my_half = (half_tiles + xcd) >> 3;
-  const int over = my_full % slots;
-  const int cut = HALVES && my_full > slots && 2 * over + my_half <= slots ? over : 0;
-  p.live = local < my_full + cut + my_half;
-  p.spares = 8 * (per - ((full_tiles + 7) >> 3) - ((half_tiles + 7) >> 3) - (HALVES ? slots / 2 : 0));
-  p.spare = -1;
-  if (!p.live) {
-    const int spare = 8 * (local - my_full - cut - my_half) + xcd;
-    if (spare < p.spares) p.spare = spare;
-    return p;
-  }
-  // the tile among those of its kind: whole eighths before this XCD's, of which the first (last) few have one more
-  const bool small = HALVES && local >= my_full + cut;
-  const bool halved = local >= my_full - cut && !small && cut > 0;
-  const int nth = small ? local - my_full - cut : halved ? my_full - cut + ((local - my_full + cut) >> 1) : local;
-  const bool second = halved && ((local - my_full + cut) & 1);
-  const int idx = small ? xcd * (half_tiles >> 3) + max(0, xcd - 8 + (half_tiles & 7)) + nth
-                        : xcd * (full_tiles >> 3) + min(xcd, full_tiles & 7) + nth;
-  constexpr int BAND = 4;
-  const int mtiles = small ? half : full;
-  const int band = idx / (BAND * ntiles), at = idx - band * BAND * ntiles;
-  const int bm = min(BAND, mtiles - band * BAND);
-  const int mt = band * BAND + at % bm;
-  p.nt = at / bm;
-  auto halve = [&] {
-    if (second) p.m0 += BM / 2;
-    else if (halved) p.hi = min(p.hi, p.m0 + BM / 2);
-    p.live = p.m0 < p.hi;
-  };
+  const Pick t = pick_tile<HALVES>(p, full, half, ntiles, bid, nbid, slots);
+  if (!p.live) return p;
   if (!offsets) {
-    p.e = 0; p.lo = 0; p.hi = rows; p.m0 = mt * BM;
-    halve();
+    p.e = 0; p.lo = 0; p.hi = rows;
+    tile_rows<BM>(p, t, 0, full);
     return p;
   }
   int before = 0;
@@ -177,31 +130,22 @@ __device__ __forceinline__ Place place_tile(const int* __restrict__ offsets, int
   for (int base = 0;; base += 64) {
     if (groups > 64) {
       s = lane_span(offsets, groups, rows, base, &carry);
-      upto_full = lane_prefix_sum(fulls(s.hi - s.lo));
-      if (HALVES) upto_half = lane_prefix_sum(halves(s.hi - s.lo));
+      upto_full = lane_prefix_sum(full_tiles_of<BM, HALVES>(s.hi - s.lo));
+      if (HALVES) upto_half = lane_prefix_sum(half_tiles_of<BM, HALVES>(s.hi - s.lo));
     }
-    const int upto = small ? upto_half : upto_full;
-    const unsigned long long has = __ballot(before + upto > mt);
+    const int upto = t.small ? upto_half : upto_full;
+    const unsigned long long has = __ballot(before + upto > t.mt);
     if (has) {
       const int l = __builtin_ctzll(has);
       p.e = base + l;
       p.lo = __builtin_amdgcn_readlane(s.lo, l);
       p.hi = __builtin_amdgcn_readlane(s.hi, l);
-      const int mine = fulls(p.hi - p.lo);
-      p.m0 = p.lo + (small ? mine : mt - (before + __builtin_amdgcn_readlane(upto, l) - mine)) * BM;
-      halve();
+      const int mine = full_tiles_of<BM, HALVES>(p.hi - p.lo);
+      tile_rows<BM>(p, t, before + __builtin_amdgcn_readlane(upto, l) - mine, mine);
       return p;
     }
     before += __builtin_amdgcn_readlane(upto, 63);
   }
-}
-
-// The largest number of workgroups that place_tile can need, with some to spare that clear rows; 0: too many.
-// `cut`: tiles of an XCD that may be made as halves.
-inline unsigned place_grid(int BM, int groups, bool ragged, int rows, int ntiles, int cut) {
-  const long long mt = ragged ? (long long)rows / BM + (groups < rows ? groups : rows) : ((long long)rows + BM - 1) / BM;
-  const long long n = ((mt * ntiles + 7) / 8 + cut + (ragged ? 8 : 0)) * 8;
-  return n < (1ll << 30) ? (unsigned)n : 0u;
 }
 
 // Rows in no group := 0, by the workgroups that have no tile.
@@ -456,12 +400,13 @@ struct Store {
   }
 };
 
-// Rounds in which `slots` resident workgroups make that many tiles.  The last one, where it is half empty or more, is made
-// of halves (place_tile).
+// Rounds in which `slots` resident workgroups make that many tiles.  A last one that is at most half full is made of halves
+// (products_place.h), two workgroups a tile: 0.39 to 0.41 of a round where it is an eighth to a quarter full, 0.54 where it is
+// half full (4500, 5000 and 6000 x 4096 in 256 x 256 tiles, contractions of 4096 in bf16 and in 8 bits).
 inline double rounds_of(double tiles, double slots, bool halves) {
   if (tiles <= slots) return 1.0;
   const double whole = (double)(long long)(tiles / slots), rest = tiles / slots - whole;
-  return whole + (rest < 0.02 ? 0.0 : halves && rest <= 0.5 ? 0.7 : 1.0);
+  return whole + (rest < 0.02 ? 0.0 : halves && rest <= 0.5 ? 0.35 + 0.4 * rest : 1.0);
 }
 
 // Workgroups with this much LDS that an XCD of this process holds at a time.
