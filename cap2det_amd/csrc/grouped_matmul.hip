@@ -220,24 +220,27 @@ __global__ __launch_bounds__(WM * WN * KG * 64, 2) void grouped_wgrad_kernel(Wgr
   S::run(acc, smem + wave * S::BYTES, (char*)dw, a.k * 4ll, a.n - n, a.k - k, a.accumulate);
 }
 
-// dw (+)= the sum of the shares' tiles, in their order.
+// dw (+)= the sum of the shares' tiles, in their order.  What dw holds is added last, as by a workgroup that made the whole
+// gradient: added first, shares below half a step of a large dw would go one by one.
 __global__ __launch_bounds__(256) void join_shares_kernel(const float* __restrict__ parts, float* __restrict__ dw, long long count,
                                                           int splits, int accumulate) {
   for (long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 4; i < count; i += (long long)gridDim.x * 1024) {
     if (i + 4 <= count) {
-      f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-      if (accumulate) __builtin_memcpy(&v, dw + i, 16);
+      f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f}, p;
       for (int s = 0; s < splits; ++s) {
-        f32x4 p;
         __builtin_memcpy(&p, parts + s * count + i, 16);
+        v += p;
+      }
+      if (accumulate) {
+        __builtin_memcpy(&p, dw + i, 16);
         v += p;
       }
       store_at((char*)(dw + i), v);
     } else {
       for (long long j = i; j < count; ++j) {
-        float v = accumulate ? dw[j] : 0.0f;
+        float v = 0.0f;
         for (int s = 0; s < splits; ++s) v += parts[s * count + j];
-        dw[j] = v;
+        dw[j] = accumulate ? v + dw[j] : v;
       }
     }
   }
