@@ -1020,11 +1020,15 @@ def _fp8_product(a, a_scale, b, b_scale, offsets, groups, rows, n, k, out, out_d
 
 
 def fp8_matmul(a, a_scale, b, b_scale, out=None, out_dtype=torch.bfloat16, bias=None, relu=False):
-  """act(a . b^T + bias) of block-scaled 8-bit matrices with fp32 sums: a [rows, k] with a_scale
+  """act(a . b^T + bias) of block-scaled 8-bit matrices: a [rows, k] with a_scale
   [rows, ceil(k / 128)] (fp8_quantize, block_rows 1; float8_e4m3fn, or float8_e5m2 as gradients use), b
   [n, k] float8_e4m3fn with b_scale [ceil(n / 128), ceil(k / 128)] (block_rows 128), bias [n] fp32 ->
   [rows, n] bf16 or fp32.  The two scales of a block are multiplied first, as fp32.  The input gradient is the same
-  product on the transposed weight."""
+  product on the transposed weight.
+
+  An fp32 result has fp32 sums.  For a bf16 result the products of 8 consecutive k are cut off at 2^-13 of the largest
+  of them (factors below their type's least normal value count as that), and what follows is fp32: where large products
+  of 8 k cancel, at most 7 * 2^-13 of the largest is lost of the rest.  Ask for an fp32 result where that matters."""
   device = _device()
   if not (bias is None and _tensors(a, a_scale, b, b_scale) and a.dim() == 2 and b.dim() == 2 and
           a.get_device() == b.get_device() == a_scale.get_device() == b_scale.get_device() == device and
