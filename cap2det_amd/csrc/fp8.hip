@@ -142,6 +142,7 @@ struct QuantArgs {
   float* scale;
   int rows, cols, kb;
   int span, per_wg;            // 1 x 128 blocks, and rows, of a workgroup
+  int row_wg, col_wg, batch0;  // where this launch begins: workgroups along the rows and the columns, matrix of the stack
   unsigned magic;              // ceil(2^32 / kb): t / kb = umulhi(t, magic) for t < 2^16
 };
 
@@ -151,12 +152,12 @@ struct QuantArgs {
 template <class T, bool E5M2>
 __global__ __launch_bounds__(256) void quantize_rows_kernel(QuantArgs a) {
   const int lane16 = threadIdx.x & 15, slot = threadIdx.x >> 4;
-  const long long row0 = (long long)blockIdx.x * a.per_wg;
+  const long long row0 = (long long)(a.row_wg + blockIdx.x) * a.per_wg, matrix = a.batch0 + blockIdx.z;
   const bool wide = a.kb > a.span;  // a row is several workgroups'
-  const int j0 = blockIdx.y * a.span, nj = min(a.span, a.kb - j0);
+  const int j0 = (a.col_wg + blockIdx.y) * a.span, nj = min(a.span, a.kb - j0);
   const int rows = (int)min((long long)a.per_wg, a.rows - row0);
   const int tasks = wide ? nj : rows * a.kb;
-  const T* x = (const T*)a.x + blockIdx.z * a.x_batch;
+  const T* x = (const T*)a.x + matrix * a.x_batch;
   float v[4][8];
 #pragma unroll
   for (int u = 0; u < 4; ++u) {
@@ -174,7 +175,7 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(QuantArgs a) {
       const int r = wide ? 0 : a.kb == 1 ? t : (int)__umulhi((unsigned)t, a.magic);
       const int j = wide ? j0 + t : t - r * a.kb;
       const float m = largest_of_16_lanes(largest(v[u])), s = scale_of<E5M2>(m);
-      const long long row = (long long)blockIdx.z * a.rows + row0 + r;
+      const long long row = matrix * a.rows + row0 + r;
       store_chunk(a.q + row * a.cols, j * 128 + lane16 * 8, a.cols, quantize8<T, E5M2>(v[u], m, s));
       if (lane16 == 0) a.scale[row * a.kb + j] = s;
     }
@@ -191,7 +192,8 @@ __global__ __launch_bounds__(2048 / U) void quantize_square_kernel(QuantArgs a) 
   const int mb = (a.rows + 127) / 128;
   const int bj = blockIdx.x % a.kb, bi = blockIdx.x / a.kb;
   const int c = bj * 128 + lane16 * 8;
-  const T* x = (const T*)a.x + blockIdx.y * a.x_batch;
+  const long long matrix = a.batch0 + blockIdx.y;
+  const T* x = (const T*)a.x + matrix * a.x_batch;
   float v[U][8], m = 0.0f;
 #pragma unroll
   for (int u = 0; u < U; ++u) {
@@ -215,30 +217,45 @@ __global__ __launch_bounds__(2048 / U) void quantize_square_kernel(QuantArgs a) 
   for (int u = 0; u < U; ++u) {
     const int r = bi * 128 + slot + STEP * u;
     if (r < a.rows)
-      store_chunk(a.q + ((long long)blockIdx.y * a.rows + r) * a.cols, c, a.cols, quantize8<T, E5M2>(v[u], m, s));
+      store_chunk(a.q + (matrix * a.rows + r) * a.cols, c, a.cols, quantize8<T, E5M2>(v[u], m, s));
   }
-  if (threadIdx.x == 0) a.scale[((long long)blockIdx.y * mb + bi) * a.kb + bj] = s;
+  if (threadIdx.x == 0) a.scale[(matrix * mb + bi) * a.kb + bj] = s;
 }
 
+// A launch holds fewer than 2^32 threads along x and 2^16 workgroups along y and z: what is larger goes in several.
 template <class T, bool E5M2>
 int launch_quantize(QuantArgs a, int batch, int block_rows, hipStream_t stream) {
+  constexpr long long X = 1 << 22, YZ = 65535;
+  auto least = [](long long n, long long most) { return (unsigned)(n < most ? n : most); };
   if (block_rows == 1) {
-    const long long blocks = (long long)batch * a.rows * a.kb;
+    const double blocks = (double)batch * a.rows * a.kb;
     a.span = blocks >= 64 * 512 ? 64 : blocks >= 32 * 512 ? 32 : 16;
     a.per_wg = a.kb >= a.span ? 1 : a.span / a.kb;
-    const long long gx = ((long long)a.rows + a.per_wg - 1) / a.per_wg;
-    const int gy = (a.kb + a.span - 1) / a.span;
-    if (gx >= (1ll << 31) || gy > 65535 || batch > 65535) return C2D_ERR_UNSUPPORTED;
-    hipLaunchKernelGGL((quantize_rows_kernel<T, E5M2>), dim3((unsigned)gx, gy, batch), dim3(256), 0, stream, a);
-  } else {
-    const long long gx = ((long long)a.rows + 127) / 128 * a.kb;
-    if (gx >= (1ll << 31) || batch > 65535) return C2D_ERR_UNSUPPORTED;
-    if (gx * batch < c2d_available_cus())
-      hipLaunchKernelGGL((quantize_square_kernel<T, E5M2, 2>), dim3((unsigned)gx, batch), dim3(1024), 0, stream, a);
-    else
-      hipLaunchKernelGGL((quantize_square_kernel<T, E5M2, 8>), dim3((unsigned)gx, batch), dim3(256), 0, stream, a);
+    const long long gx = ((long long)a.rows + a.per_wg - 1) / a.per_wg, gy = (a.kb + a.span - 1) / a.span;
+    for (long long z = 0; z < batch; z += YZ)
+      for (long long y = 0; y < gy; y += YZ)
+        for (long long x = 0; x < gx; x += X) {
+          a.row_wg = (int)x;
+          a.col_wg = (int)y;
+          a.batch0 = (int)z;
+          hipLaunchKernelGGL((quantize_rows_kernel<T, E5M2>), dim3(least(gx - x, X), least(gy - y, YZ), least(batch - z, YZ)),
+                             dim3(256), 0, stream, a);
+          if (c2d_launch_status() != C2D_OK) return C2D_ERR_LAUNCH;
+        }
+    return C2D_OK;
   }
-  return c2d_launch_status();
+  const long long gx = ((long long)a.rows + 127) / 128 * a.kb;
+  if (gx >= (1ll << 24)) return C2D_ERR_UNSUPPORTED;  // (415 GB and more of one bf16 matrix and its values)
+  for (long long z = 0; z < batch; z += YZ) {
+    a.batch0 = (int)z;
+    const dim3 grid((unsigned)gx, least(batch - z, YZ));
+    if (gx * batch < c2d_available_cus())
+      hipLaunchKernelGGL((quantize_square_kernel<T, E5M2, 2>), grid, dim3(1024), 0, stream, a);
+    else
+      hipLaunchKernelGGL((quantize_square_kernel<T, E5M2, 8>), grid, dim3(256), 0, stream, a);
+    if (c2d_launch_status() != C2D_OK) return C2D_ERR_LAUNCH;
+  }
+  return C2D_OK;
 }
 
 }  // namespace
@@ -260,7 +277,7 @@ extern "C" int c2dp_fp8_quantize(const void* x, int x_type, long long ldx, long 
   a.rows = rows;
   a.cols = cols;
   a.kb = (int)(((long long)cols + 127) / 128);
-  a.span = a.per_wg = 0;
+  a.span = a.per_wg = a.row_wg = a.col_wg = a.batch0 = 0;
   a.magic = (unsigned)((0x100000000ull + a.kb - 1) / a.kb);
   const int es = x_type == C2DP_F32 ? 4 : 2;
   const hipStream_t s = (hipStream_t)stream;
@@ -478,7 +495,7 @@ __global__ __launch_bounds__(WM * WN * KG * 64, 2) void fp8_tile_kernel(FewArgs 
   typedef Fp8Tiles<E5M2, WM, WN, MT, NT, KG, D, VEC> C;
   __shared__ __attribute__((aligned(1024))) char smem[KG * C::RING];
   typedef typename std::conditional<OUT16, __bf16, float>::type out_t;
-  const Place p = place_tile<C::BM, (MT > 1)>(a.offsets, a.groups, a.rows, a.ntiles, blockIdx.x, gridDim.x, a.slots);
+  const Place p = place_tile<C::BM, (MT > 1)>(a.offsets, a.groups, a.rows, a.ntiles, workgroup(), workgroups(), a.slots);
   if (!p.live) {
     if (a.clear) clear_rest(p, (out_t*)a.y, a.ldy, a.rows, a.n, C::NTH * KG);
     return;
@@ -500,7 +517,7 @@ int launch_tiles(FewArgs a, hipStream_t stream) {
   a.slots = slots_per_xcd(KG * Fp8Tiles<E5M2, WM, WN, MT, NT, KG, D, VEC>::RING);
   const unsigned grid = place_grid(BM, a.groups, a.offsets != nullptr, a.rows, a.ntiles, MT > 1 ? a.slots / 2 : 0);
   if (!grid) return C2D_ERR_UNSUPPORTED;
-  hipLaunchKernelGGL((fp8_tile_kernel<E5M2, WM, WN, MT, NT, KG, D, VEC, OUT16>), dim3(grid), dim3(WM * WN * KG * 64), 0, stream, a);
+  hipLaunchKernelGGL((fp8_tile_kernel<E5M2, WM, WN, MT, NT, KG, D, VEC, OUT16>), grid_of(grid), dim3(WM * WN * KG * 64), 0, stream, a);
   return c2d_launch_status();
 }
 

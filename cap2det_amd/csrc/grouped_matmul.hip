@@ -165,7 +165,7 @@ __global__ __launch_bounds__(WM * WN * KG * 64, 2) void grouped_rows_kernel(FewA
   typedef Core<ES, false, TRB, WM, WN, MT, NT, KG, D, VEC> C;
   __shared__ __attribute__((aligned(1024))) char smem[KG * C::RING];
   typedef typename std::conditional<OUT16, __bf16, float>::type out_t;
-  const Place p = place_tile<C::BM, (MT > 1)>(a.offsets, a.groups, a.rows, a.ntiles, blockIdx.x, gridDim.x, a.slots);
+  const Place p = place_tile<C::BM, (MT > 1)>(a.offsets, a.groups, a.rows, a.ntiles, workgroup(), workgroups(), a.slots);
   if (!p.live) {
     if (a.clear) clear_rest(p, (out_t*)a.y, a.ldy, a.rows, a.n, C::NTH * KG);
     return;
@@ -190,7 +190,8 @@ __global__ __launch_bounds__(WM * WN * KG * 64, 2) void grouped_wgrad_kernel(Wgr
   // about 512 x 2048 x 2048: 242 us; tiles in their order 252, 576 MB fetched of 134; an eighth of all tiles 271.  One
   // group of 16384 x 2048 x 2048: 138 us, in their order 165).
   const int tiles = a.ntiles * a.ktiles, total = tiles * a.splits * a.groups;
-  const int xcd = blockIdx.x & 7, window = blockIdx.x >> 8 << 8, at_xcd = blockIdx.x >> 3 & 31;
+  const unsigned wg = workgroup();
+  const int xcd = wg & 7, window = wg >> 8 << 8, at_xcd = wg >> 3 & 31;
   const int here = min(256, total - window), share = (here + 7) >> 3;
   if (at_xcd >= share || xcd * share + at_xcd >= here) return;
   const int idx = window + xcd * share + at_xcd;
@@ -326,7 +327,7 @@ int launch_tiles(FewArgs a, hipStream_t stream) {
   a.slots = slots_per_xcd(KG * Core<ES, false, TRB, WM, WN, MT, NT, KG, D, VEC>::RING);
   const unsigned grid = place_grid(BM, a.groups, true, a.rows, a.ntiles, MT > 1 ? a.slots / 2 : 0);
   if (!grid) return C2D_ERR_UNSUPPORTED;
-  hipLaunchKernelGGL((grouped_rows_kernel<ES, TRB, WM, WN, MT, NT, KG, D, VEC, OUT16>), dim3(grid), dim3(WM * WN * KG * 64), 0, stream, a);
+  hipLaunchKernelGGL((grouped_rows_kernel<ES, TRB, WM, WN, MT, NT, KG, D, VEC, OUT16>), grid_of(grid), dim3(WM * WN * KG * 64), 0, stream, a);
   return c2d_launch_status();
 }
 
@@ -409,7 +410,7 @@ int launch_wgrad(WgradArgs a, hipStream_t stream) {
   a.ktiles = (a.k + WN * NT * 32 - 1) / (WN * NT * 32);
   const long long grid = (long long)a.groups * a.ntiles * a.ktiles * a.splits;
   if (grid >= (1ll << 30)) return C2D_ERR_UNSUPPORTED;
-  hipLaunchKernelGGL((grouped_wgrad_kernel<ES, WM, WN, MT, NT, KG, D, VEC>), dim3((unsigned)((grid + 255) / 256 * 256)), dim3(WM * WN * KG * 64), 0, stream, a);
+  hipLaunchKernelGGL((grouped_wgrad_kernel<ES, WM, WN, MT, NT, KG, D, VEC>), grid_of((grid + 255) / 256 * 256), dim3(WM * WN * KG * 64), 0, stream, a);
   return c2d_launch_status();
 }
 

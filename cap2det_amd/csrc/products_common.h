@@ -91,6 +91,15 @@ __device__ __forceinline__ Span group_span(const int* __restrict__ offsets, int 
   }
 }
 
+// Workgroups by number.  A launch holds fewer than 2^32 threads along x, 2^23 workgroups of 512: more than 2^22 go along y, in
+// rows of 2^22, which keeps their way round the XCDs.
+inline dim3 grid_of(long long workgroups) {
+  constexpr long long ROW = 1 << 22;
+  return workgroups <= ROW ? dim3((unsigned)workgroups) : dim3((unsigned)ROW, (unsigned)((workgroups + ROW - 1) / ROW));
+}
+__device__ __forceinline__ unsigned workgroup() { return blockIdx.y * gridDim.x + blockIdx.x; }
+__device__ __forceinline__ unsigned workgroups() { return gridDim.y * gridDim.x; }
+
 // Tile of workgroup `bid` (products_place.h).  The host cannot know how many row tiles the groups make; it launches the
 // largest number, rows / BM + groups, and each wave counts them here: one or two loads and two dozen lane shuffles
 // for 64 groups.
@@ -153,8 +162,8 @@ template <class T>
 __device__ __forceinline__ void clear_rest(const Place& p, T* y, long long ldy, int rows, int n, int threads) {
   if (p.spare < 0) return;
   const int rest = rows - (p.end - p.begin);
-  for (int i = p.spare; i < rest; i += p.spares) {
-    const int row = i < p.begin ? i : p.end + (i - p.begin);
+  for (long long i = p.spare; i < rest; i += p.spares) {
+    const long long row = i < p.begin ? i : p.end + (i - p.begin);
     for (int c = threadIdx.x; c < n; c += threads) y[row * ldy + c] = (T)0.0f;
   }
 }

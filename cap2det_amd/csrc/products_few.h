@@ -112,7 +112,7 @@ __global__ __launch_bounds__(KW * 64) void few_rows_kernel(FewArgs p) {
   typedef typename std::conditional<OUT16, __bf16, float>::type out_t;
   constexpr int PITCH = BN + 4;  // floats; 16-byte aligned rows, rows four banks apart
   __shared__ __attribute__((aligned(16))) float part[KW][BM][PITCH];
-  const Place pl = place_tile<BM, false>(p.offsets, p.groups, p.rows, p.ntiles, blockIdx.x, gridDim.x, 1);
+  const Place pl = place_tile<BM, false>(p.offsets, p.groups, p.rows, p.ntiles, workgroup(), workgroups(), 1);
   if (!pl.live) {
     if (p.clear) clear_rest(pl, (out_t*)p.y, p.ldy, p.rows, p.n, KW * 64);
     return;
@@ -235,7 +235,7 @@ int launch_few(FewArgs p, hipStream_t stream) {
   p.ntiles = (p.n + 16 * NT - 1) / (16 * NT);
   const unsigned grid = place_grid(16 * MT, p.groups, p.offsets != nullptr, p.rows, p.ntiles, 0);
   if (!grid) return C2D_ERR_UNSUPPORTED;
-  hipLaunchKernelGGL((few_rows_kernel<KIND, E5M2, MT, NT, KW, VEC, OUT16>), dim3(grid), dim3(KW * 64), 0, stream, p);
+  hipLaunchKernelGGL((few_rows_kernel<KIND, E5M2, MT, NT, KW, VEC, OUT16>), grid_of(grid), dim3(KW * 64), 0, stream, p);
   return c2d_launch_status();
 }
 

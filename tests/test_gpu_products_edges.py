@@ -73,3 +73,82 @@ def test_small_products_beside_large_ones_that_cancel(a_type, m, n, k):
     tol = tol + _cut(a.float()[:, at], b.float()[:, at], 2.0 ** (-6 if a_type == E4M3 else -14)) * a_s[:, c, None] * up.spread(
         b_s[:, c, None].expand(-1, 1), 128, (n, 1)).t()
   up.assert_within(ops.fp8_matmul(a, a_s, b, b_s), want, tol + up.half_step(BF16) * (want.abs() + tol))
+
+
+# Sizes whose workgroups, along one dimension of a launch, are more than it holds
+
+@pytest.mark.parametrize("rows", [1, 128])
+def test_quantize_stacks_of_many_matrices(rows):
+  gen = _gen(51)
+  x = torch.randn(70000, 8, 64, generator=gen, device="cuda").to(BF16)
+  q, s = ops.fp8_quantize(x, rows)
+  want_q, want_s = ops.fp8_quantize(x.view(-1, 64))
+  if rows == 1:
+    assert torch.equal(q.view(torch.uint8), want_q.view(torch.uint8).view(x.shape)) and torch.equal(s, want_s.view(s.shape))
+  else:
+    assert torch.equal(s, want_s.view(70000, 8, 1).amax(1, keepdim=True))
+    for e in (0, 65534, 65535, 69999):
+      assert torch.equal(q[e].view(torch.uint8), ops.fp8_quantize(x[e], 128)[0].view(torch.uint8))
+
+
+@pytest.mark.parametrize("rows", [1, 128])
+@pytest.mark.parametrize("m,k", [((1 << 30) - 77, 1), (1, 600000007)])
+def test_quantize_long_and_wide_matrices(rows, m, k):
+  """2^30 rows of one column; more column blocks of a row than a launch has workgroups along y.  Values +-1 and, now and
+  then, 2: a block's largest is 1 or 2, 448 or 224 its ones."""
+  if torch.cuda.mem_get_info()[0] < 60 << 30:
+    pytest.skip("needs 60 GB")
+  x = torch.ones(m, k, device="cuda", dtype=BF16)
+  flat = x.view(-1)
+  flat[::3] = -1
+  flat[7::100003] = 2
+  q, s = ops.fp8_quantize(x, rows)
+  of_scale = 128 if k > 1 else rows                          # elements along the long side that share a scale
+  n = flat.numel()
+  whole = n // of_scale * of_scale
+  top = flat[:whole].view(-1, of_scale).abs().amax(1).float()
+  if whole < n:
+    top = torch.cat([top, flat[whole:].abs().amax().float()[None]])
+  assert torch.equal(s.view(-1), (top.double() / 448).float())
+  for lo in range(0, n, of_scale << 20):
+    part = flat[lo:lo + (of_scale << 20)].float()
+    share = top[lo // of_scale:][:-(-part.numel() // of_scale)].repeat_interleave(of_scale)[:part.numel()]
+    got = q.view(torch.uint8).view(-1)[lo:lo + part.numel()].view(E4M3).float()
+    assert torch.equal(got, part * 448 / share), lo
+
+
+def test_products_of_more_row_tiles_than_a_launch_has_along_x():
+  """2^28 rows: 2^23 and 2^22 tiles and some.  Every row is one of eight, each result row one of eight."""
+  if torch.cuda.mem_get_info()[0] < 60 << 30:
+    pytest.skip("needs 60 GB")
+  gen = _gen(52)
+  t, n, k = (1 << 28) + 1000, 16, 16
+  offsets = [3, (1 << 27) + 5, (1 << 27) + 5, t - 50]
+  few = up.integers(gen, (8, k), 4, BF16)
+  w = up.integers(gen, (3, n, k), 4, BF16)
+  x = few.repeat(t // 8, 1)
+  offs = _offs(offsets)
+
+  def check(y, want_of):
+    assert (y[:3] == 0).all() and (y[t - 50:] == 0).all()
+    for e, (lo, hi) in enumerate(up.spans(offsets, t)):
+      for at in range(lo, hi, 1 << 25):
+        part = y[at:min(hi, at + (1 << 25))]
+        want = want_of(e).roll(-(at % 8), 0)
+        whole = part.shape[0] // 8 * 8
+        assert (part[:whole].view(-1, 8, part.shape[1]) == want).all() and (part[whole:] == want[:part.shape[0] - whole]).all()
+
+  exact = lambda a, b: (a.double() @ b.double()).to(BF16)
+  check(ops.grouped_matmul(x, w, offs), lambda e: exact(few, w[e].t()))
+  check(ops.grouped_matmul_dgrad(x, w, offs), lambda e: exact(few, w[e]))
+  at = torch.tensor([0, 2, 3, 4, 1000003, offsets[1] - 1, offsets[1], (1 << 27) + 6, t - 51, t - 50], device="cuda")
+  dy = torch.zeros(t, 8, device="cuda", dtype=BF16)
+  dy[at] = up.integers(gen, (len(at), 8), 4, BF16)
+  dw = torch.zeros(3, 8, k, dtype=torch.float64, device="cuda")
+  for r in at.tolist():
+    for e, (lo, hi) in enumerate(up.spans(offsets, t)):
+      if lo <= r < hi:
+        dw[e] += dy[r].double()[:, None] * x[r].double()
+  assert torch.equal(ops.grouped_matmul_wgrad(x, dy, offs), dw.float())
+  q, s = x.to(E4M3), torch.ones(t, 1, device="cuda")
+  check(ops.grouped_matmul_fp8(q, s, w.to(E4M3), torch.ones(3, 1, 1, device="cuda"), offs), lambda e: exact(few, w[e].t()))
