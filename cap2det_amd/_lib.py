@@ -30,6 +30,10 @@ class Cap2DetHipError(RuntimeError):
   """Raised when a C-ABI call returns a negative C2D_ERR_* code."""
 
 
+class UnsupportedError(Cap2DetHipError, ValueError):
+  """C2D_ERR_UNSUPPORTED: valid arguments of sizes that the call does not take."""
+
+
 def _ctype(decl):
   decl = decl.strip()
   if "*" in decl:
@@ -111,7 +115,7 @@ def load():
 def check(code, what):
   if code != 0:
     msg = load().c2d_error_string(int(code)).decode()
-    raise Cap2DetHipError("%s failed: %s (%d)" % (what, msg, code))
+    raise (UnsupportedError if code == -2 else Cap2DetHipError)("%s failed: %s (%d)" % (what, msg, code))
 
 
 # The step-plan recorder (cap2det_amd/step_plan.py) while a step is being recorded, else None: every

@@ -843,7 +843,7 @@ def x9_planes(t):
 # not read; in a result they are zero, or, where `out` is given, left as they were.  `out` has to lie outside the
 # memory that the operands span, gaps between their rows included.
 #
-# Matrices may be row-strided views (columns contiguous).  Everything is queued on the current stream of the
+# Matrices may be row-strided views (columns contiguous), with rows of operands up to 4 MiB apart.  Everything is queued on the current stream of the
 # current device, where the tensors have to be; results and workspaces of one call are the call's own, so
 # that calls on several streams and graphs captured into memory pools of their own share none.  A step plan
 # keeps those of the calls that it recorded, since it holds their addresses.
@@ -852,6 +852,7 @@ FP8_BLOCK = 128
 FP8_TYPES = (torch.float8_e4m3fn, torch.float8_e5m2)
 _WIDE_TYPES = (torch.float32, torch.bfloat16)
 _MAX_SIZE = 1 << 30
+_MAX_PITCH = 1 << 22        # bytes
 _PRODUCT_TYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float8_e4m3fn: 2, torch.float8_e5m2: 3}
 
 
@@ -886,6 +887,11 @@ def _operand(t, name, types, dims, device):
 def _check_sizes(*sizes):
   if max(sizes) > _MAX_SIZE:
     raise ValueError("rows, columns and groups up to %d, got %d" % (_MAX_SIZE, max(sizes)))
+
+
+def _check_pitch(t, name, step):
+  if step * t.element_size() > _MAX_PITCH:
+    raise ValueError("%s: rows up to %d bytes apart are taken, got %d" % (name, _MAX_PITCH, step * t.element_size()))
 
 
 def _whole(t, name, types, shape, device):
@@ -1003,6 +1009,10 @@ def _check_fp8(a, a_scale, b, b_scale, offsets, bias, dense):
 
 def _fp8_product(a, a_scale, b, b_scale, offsets, groups, rows, n, k, out, out_dtype, bias, relu):
   _check_sizes(groups, rows, n, k)
+  lda = _pitch(a, "a")
+  if (lda > _MAX_PITCH or k > _MAX_PITCH) and rows and n:
+    _check_pitch(a, "a", lda)
+    _check_pitch(b, "b", k)
   if out is None:
     if out_dtype is not _BF16 and out_dtype is not _F32:
       raise ValueError("out_dtype: one of %s is wanted, got %s" % (_names(_WIDE_TYPES), out_dtype))
@@ -1012,7 +1022,7 @@ def _fp8_product(a, a_scale, b, b_scale, offsets, groups, rows, n, k, out, out_d
     _given_result(y, (rows, n), _WIDE_TYPES, _device(), (a, a_scale, b, b_scale, bias, offsets))
     ldy = _pitch(y, "out")
   if rows and n:
-    _lib.call("c2dp_fp8_matmul", a.data_ptr(), _PRODUCT_TYPE[a.dtype], _pitch(a, "a"), a_scale.data_ptr(), b.data_ptr(),
+    _lib.call("c2dp_fp8_matmul", a.data_ptr(), _PRODUCT_TYPE[a.dtype], lda, a_scale.data_ptr(), b.data_ptr(),
               b_scale.data_ptr(), None if offsets is None else offsets.data_ptr(), groups,
               None if bias is None else bias.data_ptr(), 1 if relu else 0, y.data_ptr(), _PRODUCT_TYPE[y.dtype], ldy,
               rows, n, k, clear, _stream())
@@ -1081,6 +1091,10 @@ def _grouped_rows(entry, x, name, w, offsets, out, out_dtype, dgrad):
   groups, n, k = w.shape
   rows, wide = x.shape[0], k if dgrad else n
   _check_sizes(groups, rows, n, k)
+  ldx = _pitch(x, name)
+  if (ldx > _MAX_PITCH // 4 or k > _MAX_PITCH // 4) and rows and wide:
+    _check_pitch(x, name, ldx)
+    _check_pitch(w, "w", k)
   if out is None:
     if out_dtype is None or out_dtype is x.dtype:
       y = _own(x.new_empty((rows, wide)))
@@ -1094,7 +1108,7 @@ def _grouped_rows(entry, x, name, w, offsets, out, out_dtype, dgrad):
     _given_result(y, (rows, wide), _WIDE_TYPES if x.dtype is _BF16 else (_F32,), _device(), (x, w, offsets))
     ldy = _pitch(y, "out")
   if rows and wide:
-    _lib.call(entry, x.data_ptr(), _PRODUCT_TYPE[x.dtype], _pitch(x, name), w.data_ptr(), offsets.data_ptr(), groups,
+    _lib.call(entry, x.data_ptr(), _PRODUCT_TYPE[x.dtype], ldx, w.data_ptr(), offsets.data_ptr(), groups,
               y.data_ptr(), _PRODUCT_TYPE[y.dtype], ldy, rows, n, k, clear, _stream())
   return y
 
@@ -1133,6 +1147,10 @@ def grouped_matmul_wgrad(x, dy, offsets, out=None, accumulate=False):
   rows, k = x.shape
   n, groups = dy.shape[1], offsets.shape[0] - 1
   _check_sizes(groups, rows, n, k)
+  ldx, lddy = _pitch(x, "x"), _pitch(dy, "dy")
+  if ldx > _MAX_PITCH // 4 or lddy > _MAX_PITCH // 4:
+    _check_pitch(x, "x", ldx)
+    _check_pitch(dy, "dy", lddy)
   if out is None:
     if accumulate:
       raise ValueError("accumulate: there is no `out` to add to")
@@ -1144,8 +1162,8 @@ def grouped_matmul_wgrad(x, dy, offsets, out=None, accumulate=False):
   if n and k:
     nbytes = _wgrad_workspace_bytes(groups, rows, n, k, _PRODUCT_TYPE[x.dtype])
     ws = _own(x.new_empty(nbytes, dtype=torch.uint8)) if nbytes else None
-    _lib.call("c2dp_grouped_matmul_wgrad", x.data_ptr(), _PRODUCT_TYPE[x.dtype], _pitch(x, "x"), dy.data_ptr(),
-              _pitch(dy, "dy"), offsets.data_ptr(), groups, dw.data_ptr(), rows, n, k, 1 if accumulate else 0,
+    _lib.call("c2dp_grouped_matmul_wgrad", x.data_ptr(), _PRODUCT_TYPE[x.dtype], ldx, dy.data_ptr(),
+              lddy, offsets.data_ptr(), groups, dw.data_ptr(), rows, n, k, 1 if accumulate else 0,
               None if ws is None else ws.data_ptr(), nbytes, _stream())
   return dw
 
