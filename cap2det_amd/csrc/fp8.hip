@@ -267,7 +267,7 @@ extern "C" int c2dp_fp8_quantize(const void* x, int x_type, long long ldx, long 
   C2D_CHECK_ARG(batch >= 0 && rows >= 0 && cols >= 0 && ldx >= cols && (block_rows == 1 || block_rows == 128));
   if (batch == 0 || rows == 0 || cols == 0) return C2D_OK;
   C2D_CHECK_ARG(x && q && scale);
-  if (!sizes_fit(batch, rows, cols, 0)) return C2D_ERR_UNSUPPORTED;
+  if (!sizes_fit(batch, rows, cols)) return C2D_ERR_UNSUPPORTED;
   QuantArgs a;
   a.x = x;
   a.ldx = ldx;
@@ -568,7 +568,7 @@ extern "C" int c2dp_fp8_matmul(const void* a_, int a_type, long long lda, const 
   C2D_CHECK_ARG(groups > 0 && (offsets || groups == 1) && rows >= 0 && n >= 0 && k >= 0 && lda >= k && ldy >= n);
   if (rows == 0 || n == 0) return C2D_OK;
   C2D_CHECK_ARG(y && (k == 0 || (a_ && b && a_scale && b_scale)));
-  if (!sizes_fit(groups, rows, n, k) || lda > C2DP_MAX_PITCH || k > C2DP_MAX_PITCH) return C2D_ERR_UNSUPPORTED;
+  if (!groups_fit(groups) || !sizes_fit(rows, n, k) || lda > C2DP_MAX_PITCH || k > C2DP_MAX_PITCH) return C2D_ERR_UNSUPPORTED;
   FewArgs a;
   a.a = (const char*)a_;
   a.lda = lda;

@@ -356,7 +356,7 @@ int rows_product(const void* x, int x_type, long long ldx, const void* w, const 
   if (rows == 0 || n == 0) return C2D_OK;
   C2D_CHECK_ARG(offsets && y && (contraction == 0 || (x && w)));
   const int es = x_type == C2DP_BF16 ? 2 : 4, ys = y_type == C2DP_BF16 ? 2 : 4;
-  if (!sizes_fit(groups, rows, n, k)) return C2D_ERR_UNSUPPORTED;
+  if (!groups_fit(groups) || !sizes_fit(rows, n, k)) return C2D_ERR_UNSUPPORTED;
   if ((long long)(contraction > 0 ? ldx : 1) * es > C2DP_MAX_PITCH || (long long)(k > 0 ? k : 1) * es > C2DP_MAX_PITCH)
     return C2D_ERR_UNSUPPORTED;
   FewArgs a = {};
@@ -433,7 +433,7 @@ extern "C" int c2dp_grouped_matmul_wgrad(const void* x, int x_type, long long ld
   if (n == 0 || k == 0) return C2D_OK;
   C2D_CHECK_ARG(offsets && dw && (rows == 0 || (x && dy)));
   const int es = x_type == C2DP_BF16 ? 2 : 4;
-  if (!sizes_fit(groups, rows, n, k) || ldx * es > C2DP_MAX_PITCH || lddy * es > C2DP_MAX_PITCH) return C2D_ERR_UNSUPPORTED;
+  if (!groups_fit(groups) || !sizes_fit(rows, n, k) || ldx * es > C2DP_MAX_PITCH || lddy * es > C2DP_MAX_PITCH) return C2D_ERR_UNSUPPORTED;
   const unsigned long long need = c2dp_grouped_matmul_wgrad_workspace_bytes(groups, rows, n, k, x_type);
   if (workspace_bytes < need || (need && !workspace)) return C2D_ERR_WORKSPACE;
   C2D_CHECK_ARG(((unsigned long long)workspace & 15) == 0);

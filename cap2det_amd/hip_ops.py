@@ -843,7 +843,7 @@ def x9_planes(t):
 # not read; in a result they are zero, or, where `out` is given, left as they were.  `out` has to lie outside the
 # memory that the operands span, gaps between their rows included.
 #
-# Matrices may be row-strided views (columns contiguous), with rows of operands up to 4 MiB apart.  Everything is queued on the current stream of the
+# Matrices may be row-strided views (columns contiguous), with rows of operands up to 4 MiB apart.  Up to 65536 groups.  Everything is queued on the current stream of the
 # current device, where the tensors have to be; results and workspaces of one call are the call's own, so
 # that calls on several streams and graphs captured into memory pools of their own share none.  A step plan
 # keeps those of the calls that it recorded, since it holds their addresses.
@@ -852,6 +852,7 @@ FP8_BLOCK = 128
 FP8_TYPES = (torch.float8_e4m3fn, torch.float8_e5m2)
 _WIDE_TYPES = (torch.float32, torch.bfloat16)
 _MAX_SIZE = 1 << 30
+_MAX_GROUPS = 1 << 16
 _MAX_PITCH = 1 << 22        # bytes
 _PRODUCT_TYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float8_e4m3fn: 2, torch.float8_e5m2: 3}
 
@@ -887,6 +888,11 @@ def _operand(t, name, types, dims, device):
 def _check_sizes(*sizes):
   if max(sizes) > _MAX_SIZE:
     raise ValueError("rows, columns and groups up to %d, got %d" % (_MAX_SIZE, max(sizes)))
+
+
+def _check_groups(groups):
+  if groups > _MAX_GROUPS:
+    raise ValueError("up to %d groups are taken, got %d" % (_MAX_GROUPS, groups))
 
 
 def _check_pitch(t, name, step):
@@ -1009,6 +1015,7 @@ def _check_fp8(a, a_scale, b, b_scale, offsets, bias, dense):
 
 def _fp8_product(a, a_scale, b, b_scale, offsets, groups, rows, n, k, out, out_dtype, bias, relu):
   _check_sizes(groups, rows, n, k)
+  _check_groups(groups)
   lda = _pitch(a, "a")
   if (lda > _MAX_PITCH or k > _MAX_PITCH) and rows and n:
     _check_pitch(a, "a", lda)
@@ -1091,6 +1098,7 @@ def _grouped_rows(entry, x, name, w, offsets, out, out_dtype, dgrad):
   groups, n, k = w.shape
   rows, wide = x.shape[0], k if dgrad else n
   _check_sizes(groups, rows, n, k)
+  _check_groups(groups)
   ldx = _pitch(x, name)
   if (ldx > _MAX_PITCH // 4 or k > _MAX_PITCH // 4) and rows and wide:
     _check_pitch(x, name, ldx)
@@ -1147,6 +1155,7 @@ def grouped_matmul_wgrad(x, dy, offsets, out=None, accumulate=False):
   rows, k = x.shape
   n, groups = dy.shape[1], offsets.shape[0] - 1
   _check_sizes(groups, rows, n, k)
+  _check_groups(groups)
   ldx, lddy = _pitch(x, "x"), _pitch(dy, "dy")
   if ldx > _MAX_PITCH // 4 or lddy > _MAX_PITCH // 4:
     _check_pitch(x, "x", ldx)

@@ -10,7 +10,8 @@
  *   - a pitch is at most C2DP_MAX_PITCH bytes, else C2D_ERR_UNSUPPORTED.  16-byte aligned base
  *     pointers, pitches and contraction lengths take the direct global -> LDS loads; any others are
  *     right too, through registers, and slower.
- *   - rows, n, k, cols, batch and groups are at most C2DP_MAX_SIZE, else C2D_ERR_UNSUPPORTED.
+ *   - rows, n, k, cols and batch are at most C2DP_MAX_SIZE and groups at most C2DP_MAX_GROUPS, else
+ *     C2D_ERR_UNSUPPORTED; so are the rare sizes below that which make 2^30 tiles or more.
  *   - sums are fp32, but for the products within a block of an 8-bit product with a bf16 result: see c2dp_fp8_matmul.
  *
  * Groups.  `offsets` is a DEVICE array of groups + 1 int32 row numbers: group e owns the rows
@@ -40,6 +41,7 @@ int c2dp_version(void);
 #define C2DP_BLOCK 128             /* elements of the contraction that share a scale */
 #define C2DP_MAX_PITCH (1 << 22)   /* bytes */
 #define C2DP_MAX_SIZE (1 << 30)
+#define C2DP_MAX_GROUPS (1 << 16)  /* every workgroup looks through all offsets: time grows with groups^2 */
 
 /* 8-bit values and fp32 scales of `batch` matrices x [rows][cols] (x_type C2DP_F32 or C2DP_BF16; matrix
  * i begins at x + i * x_batch elements).  Blocks are block_rows x 128, block_rows 1 or 128:

@@ -152,3 +152,22 @@ def test_products_of_more_row_tiles_than_a_launch_has_along_x():
   assert torch.equal(ops.grouped_matmul_wgrad(x, dy, offs), dw.float())
   q, s = x.to(E4M3), torch.ones(t, 1, device="cuda")
   check(ops.grouped_matmul_fp8(q, s, w.to(E4M3), torch.ones(3, 1, 1, device="cuda"), offs), lambda e: exact(few, w[e].t()))
+
+
+def test_as_many_groups_as_are_taken():
+  """65536 groups of no row, one and two, in the forward product's small tiles, its gradients' and the 8-bit product's."""
+  gen = _gen(53)
+  groups, n, k = 1 << 16, 16, 24
+  counts = torch.randint(0, 3, (groups,), generator=gen, device="cuda")
+  offs = torch.zeros(groups + 1, dtype=torch.int32, device="cuda")
+  offs[1:] = counts.cumsum(0)
+  t = int(offs[-1])
+  of = torch.arange(groups, device="cuda").repeat_interleave(counts)
+  x, dy = up.integers(gen, (t, k), 4, BF16), up.integers(gen, (t, n), 4, BF16)
+  w = up.integers(gen, (groups, n, k), 4, BF16)
+  assert torch.equal(ops.grouped_matmul(x, w, offs), (w[of].float() * x[:, None].float()).sum(-1).to(BF16))
+  assert torch.equal(ops.grouped_matmul_dgrad(dy, w, offs), (w[of].float() * dy[:, :, None].float()).sum(1).to(BF16))
+  want = torch.zeros(groups, n, k, device="cuda").index_add_(0, of, dy[:, :, None].float() * x[:, None].float())
+  assert torch.equal(ops.grouped_matmul_wgrad(x, dy, offs), want)
+  y = ops.grouped_matmul_fp8(x.to(E4M3), torch.ones(t, 1, device="cuda"), w.to(E4M3), torch.ones(groups, 1, 1, device="cuda"), offs)
+  assert torch.equal(y, (w[of].float() * x[:, None].float()).sum(-1).to(BF16))

@@ -65,6 +65,23 @@ def test_rows_at_the_largest_pitch_are_passed_on(monkeypatch):
   assert [a[2] for a in seen] == [MB4 // 2, MB4 // 2, MB4]
 
 
+def test_many_groups_are_refused(host):
+  many = (1 << 16) + 1
+  offs = torch.zeros(many + 1, dtype=torch.int32)
+  x, w = torch.zeros(2, 8, dtype=BF16), torch.zeros(many, 8, 8, dtype=BF16)
+  a, b = torch.zeros(2, 8).to(E4M3), torch.zeros(many, 8, 8, dtype=torch.uint8).view(E4M3)
+  for f in (lambda: ops.grouped_matmul(x, w, offs), lambda: ops.grouped_matmul_dgrad(x, w, offs),
+            lambda: ops.grouped_matmul_wgrad(x, x, offs),
+            lambda: ops.grouped_matmul_fp8(a, torch.ones(2, 1), b, torch.ones(many, 1, 1), offs)):
+    with pytest.raises(ValueError, match="up to 65536 groups are taken, got 65537"):
+      f()
+  lib = _lib.load()
+  assert lib.c2dp_grouped_matmul(P, 1, 8, P, P, many, P, 1, 8, 2, 8, 8, 0, None) == -2
+  assert lib.c2dp_grouped_matmul_dgrad(P, 1, 8, P, P, many, P, 1, 8, 2, 8, 8, 0, None) == -2
+  assert lib.c2dp_grouped_matmul_wgrad(P, 1, 8, P, 8, P, many, P, 2, 8, 8, 0, None, 0, None) == -2
+  assert lib.c2dp_fp8_matmul(P, 2, 8, P, P, P, P, many, None, 0, P, 1, 8, 2, 8, 8, 0, None) == -2
+
+
 def test_what_the_library_does_not_take_is_a_value_error_too():
   """65536 rows in groups of one by 2^24 columns: more tiles than are numbered."""
   with pytest.raises(ValueError, match="c2dp_grouped_matmul failed: .*-2"):
