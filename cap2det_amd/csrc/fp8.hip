@@ -521,40 +521,18 @@ int launch_tiles(FewArgs a, hipStream_t stream) {
   return c2d_launch_status();
 }
 
-// Which kernel: the one whose estimated time is least, t = rounds of resident workgroups * (us per block of k *
-// blocks + us per round), with the rates that each was measured at (us; a workgroup per CU, 128 rows of 4096 x 4096
-// and up):
-//                             a round   a block of k     measured, rows x n x k: this, and the next larger / smaller
-//   256 x 256 tiles             3.5       1.95           8192 x 8192 x 8192: 509, in 128 x 128 tiles 680
-//   128 x 128, two per CU       3.5       1.30  (0.75    1024 x 4096 x 4096:  27, in 256 x 256 tiles 53
-//                                          one per CU)    2000 x 2000 x 256:  7.4, in 64 x 64 tiles 15.7
-//   64 x 64, two K groups       3.5       0.28           256 x 4096 x 4096: 13.6, in 128 x 128 tiles 27.5
-//                                                        2000 x 416 x 1024:  6.2, in 128 x 128 tiles 10.2
-//   32 x 32 from registers      2.5       0.29           256 x 1024 x 1024:  4.9, in 64 x 64 tiles 6.0
-// Up to 16 rows a group, 16-row tiles from registers: the weights' way is all there is (1 x 8192 x 4096: 8.1 us,
-// 64 x 64 tiles 12.4; 16 x 4096 x 4096: 7.7 against 12.5).  An fp32 result doubles the matrix instructions and the
-// registers of a block's products; it has no 256 x 256 tiles, whose registers it would spill, nor have
-// operands that pass through registers on their way to LDS.
 template <bool E5M2, bool VEC, bool OUT16>
 int launch_fp8(const FewArgs& a, hipStream_t stream) {
   constexpr int KIND = OUT16 ? FP8 : FP8_WIDE;
-  const int groups = a.offsets ? min(a.groups, a.rows) : 1;
-  if ((long long)a.rows <= 16ll * groups) return launch_sixteen_rows<KIND, E5M2, VEC, OUT16>(a, stream);
-  auto tiles = [&](int side) {  // (a group's last row tile counts for what it costs, on average)
-    const double rows = a.offsets ? (double)a.rows / side + 0.4 * groups : (double)((a.rows + side - 1) / side);
-    return rows * ((a.n + side - 1) / side);
-  };
-  const double kb = a.kb, wide = OUT16 ? 1.0 : 1.5;
-  const double t256 = tiles(256), t128 = tiles(128);
-  const double us256 = rounds_of(t256, 256, true) * ((t256 <= 256 ? 1.5 : 1.95) * kb + 3.5);
-  const double us128 = rounds_of(t128, 512, true) * ((t128 <= 256 ? 0.75 : 1.3) * wide * kb + 3.5);
-  const double us64 = rounds_of(tiles(64), 256, false) * (0.28 * wide * kb + 3.5);
-  const double us32 = tiles(32) / 256 * 0.29 * kb + 2.5;
-  if (OUT16 && VEC && us256 <= us128 && us256 <= us64 && us256 <= us32)
-    return launch_tiles<E5M2, 4, 2, 2, 4, 1, 2, true, true>(a, stream);
-  if (us128 <= us64 && us128 <= us32) return launch_tiles<E5M2, 2, 2, 2, 2, 1, 2, VEC, OUT16>(a, stream);
-  if (us64 <= us32) return launch_tiles<E5M2, 2, 2, 1, 1, 2, 4, VEC, OUT16>(a, stream);
-  return launch_few<KIND, E5M2, 2, 2, 8, VEC, OUT16>(a, stream);
+  switch (fp8_shape(a.rows, a.n, a.k, a.groups, a.offsets != nullptr, OUT16, VEC)) {
+    case T16: return launch_few<KIND, E5M2, 1, 1, 8, VEC, OUT16>(a, stream);
+    case T16W: return launch_few<KIND, E5M2, 1, 2, 2, VEC, OUT16>(a, stream);
+    case T32: return launch_few<KIND, E5M2, 2, 2, 8, VEC, OUT16>(a, stream);
+    case T64: return launch_tiles<E5M2, 2, 2, 1, 1, 2, 4, VEC, OUT16>(a, stream);
+    case T256:
+      if constexpr (OUT16 && VEC) return launch_tiles<E5M2, 4, 2, 2, 4, 1, 2, true, true>(a, stream);
+    default: return launch_tiles<E5M2, 2, 2, 2, 2, 1, 2, VEC, OUT16>(a, stream);
+  }
 }
 
 }  // namespace

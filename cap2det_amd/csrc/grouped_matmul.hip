@@ -247,78 +247,7 @@ __global__ __launch_bounds__(256) void join_shares_kernel(const float* __restric
   }
 }
 
-// ---- which kernel ----------------------------------------------------------------------------------
-//
-// The one whose estimated time is least, t = rounds of resident workgroups * (us per stage * stages + us per
-// round), a stage 128 bytes of the contraction, with the rates that each was measured at:
-//   rows, bf16                    a round   a stage             measured (us)
-//   256 x 256 tiles, from half of     6      1.12 .. 1.65        8192 x 8192 x 8192: 851, in 128 x 128 tiles 1045;
-//     the CUs to all, and more                                   32 groups of 512 x 2048 x 2048: 173, 199
-//     input gradient                  6      1.3 .. 1.65         8 groups of 625 x 1000 x 1536: 29.3, 128 x 128 30.6
-//   128 x 256, in one round         3.5      0.7 .. 1.03         4500 rows of 4 groups, 1024 x 2048: 27.4, 128 x 128 29.9,
-//                                                                256 x 256 41.9; 4096 x 4096 x 4096, two rounds: 128, 256 x 256 110
-//     input gradient                3.5      0.85 .. 1.1         4292 rows of 3 groups, 1880 x 1512: 34.1, 128 x 128 38.2,
-//                                                                256 x 256 48.1
-//   128 x 128, one per CU           3.5      0.57                8 groups of 512 x 1024 x 1024: 17.4, 256 x 256 25.9,
-//     up to two, and more           3.5      0.82 .. 1.04        64 x 64 31
-//     input gradient                3.5      0.66                4096 x 2048 x 2048 in one group: 39.3, 256 x 256 48.8,
-//       up to two, and more         3.5      0.87 .. 1.15        128 x 256 37.5
-//   64 x 64, two K groups           3.0      0.25                 8 groups of 32 x 1024 x 1024: 7.0, 128 x 128 11.7
-//   32 x 32 from registers          2.5      0.29                 (forward alone)
-// Up to 16 rows a group, forward: 16 x 16 from registers.  fp32 is bound by its matrix instructions (a stage of a
-// 64 x 64 tile 0.56, of 128 x 128 1.9 or, two per CU, 3.8) and has no 256 x 256 tiles, which gain 2.5 % on
-// 4096^3 and lose wherever tiles are few (4 groups of 1024 x 416 x 1024: 241 against 42 in 64 x 64 tiles).
-enum Shape { T256, T128W, T128, T64, T32, T16 };
-Shape rows_shape(const FewArgs& a, int es, bool forward, bool vec) {
-  const int groups = a.groups < a.rows ? a.groups : a.rows;
-  if (forward && (long long)a.rows <= 16ll * groups) return T16;
-  // One group's row tiles are known.  Of several a last tile counts for what it costs, on average, and to a round of 128
-  // rows a twentieth is added, since a few tiles too many cost another one (8 groups of 625 x 1000 x 1536, input
-  // gradient, 258 tiles of 128 x 256: 33.5 us, in 256 x 256 tiles 29.3; of those more are made as halves).
-  const double spare = groups == 1 ? 1.0 : 1.05;
-  auto tiles = [&](int side, int columns) {
-    const double down = groups == 1 ? (a.rows + side - 1) / side : (double)a.rows / side + 0.4 * groups;
-    return down * ((a.n + columns - 1) / columns);
-  };
-  const double stages = ((long long)a.k * es + 127) / 128;
-  const double t256 = tiles(256, 256), t128w = tiles(128, 256), t128 = tiles(128, 128);
-  // From `lo` at half of `full` to `hi` at all of it, and behind.
-  auto between = [](double t, double full, double lo, double hi) { return t >= full ? hi : t <= full / 2 ? lo : lo + (hi - lo) * (2 * t / full - 1); };
-  const double us256 = rounds_of(t256, 256, true) * (between(t256, 256, forward ? 1.12 : 1.3, 1.65) * stages + 6.0);
-  const double us128w = spare * t128w <= 256 ? (forward ? between(t128w, 256, 0.7, 1.03) : between(t128w, 256, 0.85, 1.1)) * stages + 3.5 : 1e30;
-  const double one = es == 4 ? 1.9 : forward ? 0.57 : 0.66;
-  const double more = es == 4 ? between(t128, 512, 1.9, 3.8) : forward ? between(t128, 512, 0.82, 1.04) : between(t128, 512, 0.87, 1.15);
-  const double us128 = rounds_of(spare * t128, 512, true) * ((t128 <= 256 ? one : more) * stages + 3.5);
-  const double us64 = rounds_of(tiles(64, 64), 256, false) * ((es == 4 ? 0.56 : 0.25) * stages + 3.0);
-  const double us32 = forward ? tiles(32, 32) / 256 * (es == 4 ? 0.4 : 0.29) * stages + 2.5 : 1e30;
-  const double rest = us64 <= us32 ? us64 : us32, most = us128 <= rest ? us128 : rest;
-  if (es == 2 && vec && us256 <= us128w && us256 <= most) return T256;
-  if (es == 2 && vec && us128w <= most) return T128W;
-  if (us128 <= us64 && us128 <= us32) return T128;
-  return us64 <= us32 ? T64 : T32;
-}
-
-// Weight gradient: the same, the rows of a group the contraction, dealt to `splits` workgroups where the tiles of
-// dw are few; a round ends with the tile's way to memory, and splits with the sum over them.
-struct WgradPlan { int side, splits; };
-WgradPlan wgrad_plan(int groups, int rows, int n, int k, int es) {
-  const double stages = ((double)rows / groups * es + 127) / 128, mb = 4e-6 * groups * n * k;
-  WgradPlan best = {64, 1};
-  double least = 1e30;
-  for (int side = es == 2 ? 256 : 128; side >= 64; side /= 2) {
-    const double tiles = (double)groups * ((n + side - 1) / side) * ((k + side - 1) / side);
-    const double slots = side == 128 ? 512 : 256;
-    const double stage = es == 4 ? (side == 128 ? 3.8 : 0.56) : side == 256 ? 1.7 : side == 128 ? 1.2 : 0.27;
-    const double round = side == 256 ? 20 : side == 128 ? 11 : 4;
-    for (int splits = 1; splits == 1 || (splits <= 32 && 4 * splits <= stages && splits * mb <= 256); splits *= 2) {
-      const double one = side == 128 && tiles * splits <= 256 ? 0.6 : 1.0;  // (one workgroup per CU)
-      const double t = rounds_of(tiles * splits, slots, false) * one * (stage * stages / splits + round) +
-                       (splits > 1 ? 4.0 + (splits + 1) * mb / 4.0 : 0.0);
-      if (t < least) { least = t; best = {side, splits}; }
-    }
-  }
-  return best;
-}
+// ---- launches (products_choice.h says which) ---------------------------------------------------------
 
 template <int ES, bool TRB, int WM, int WN, int MT, int NT, int KG, int D, bool VEC, bool OUT16>
 int launch_tiles(FewArgs a, hipStream_t stream) {
@@ -333,13 +262,14 @@ int launch_tiles(FewArgs a, hipStream_t stream) {
 
 template <int ES, bool TRB, bool VEC, bool OUT16>
 int launch_rows(const FewArgs& a, hipStream_t stream) {
-  const Shape shape = rows_shape(a, ES, !TRB, VEC);
+  const Shape shape = rows_shape(a.rows, a.n, a.k, a.groups, ES, !TRB, VEC);
   if constexpr (ES == 2 && VEC) {
     if (shape == T256) return launch_tiles<ES, TRB, 2, 4, 4, 2, 1, 2, true, OUT16>(a, stream);
     if (shape == T128W) return launch_tiles<ES, TRB, 2, 4, 2, 2, 1, 2, true, OUT16>(a, stream);
   }
   if constexpr (!TRB) {
-    if (shape == T16) return launch_sixteen_rows<ES == 2 ? BF16 : F32, false, VEC, OUT16>(a, stream);
+    if (ES == 2 && shape == T16W) return launch_few<BF16, false, 1, 2, 2, VEC, OUT16>(a, stream);
+    if (shape == T16) return launch_few<ES == 2 ? BF16 : F32, false, 1, 1, 8, VEC, OUT16>(a, stream);
     if (shape == T32) return launch_few<ES == 2 ? BF16 : F32, false, 2, 2, 8, VEC, OUT16>(a, stream);
   }
   if (shape == T128) return launch_tiles<ES, TRB, 2, 2, 2, 2, 1, 2, VEC, OUT16>(a, stream);

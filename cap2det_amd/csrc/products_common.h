@@ -12,6 +12,7 @@
 #pragma once
 #include "c2d_common.h"
 #include "../../include/cap2det_products.h"
+#include "products_choice.h"
 #include "products_place.h"
 #include <type_traits>
 
@@ -408,15 +409,6 @@ struct Store {
     }
   }
 };
-
-// Rounds in which `slots` resident workgroups make that many tiles.  A last one that is at most half full is made of halves
-// (products_place.h), two workgroups a tile: 0.39 to 0.41 of a round where it is an eighth to a quarter full, 0.54 where it is
-// half full (4500, 5000 and 6000 x 4096 in 256 x 256 tiles, contractions of 4096 in bf16 and in 8 bits).
-inline double rounds_of(double tiles, double slots, bool halves) {
-  if (tiles <= slots) return 1.0;
-  const double whole = (double)(long long)(tiles / slots), rest = tiles / slots - whole;
-  return whole + (rest < 0.02 ? 0.0 : halves && rest <= 0.5 ? 0.35 + 0.4 * rest : 1.0);
-}
 
 // Workgroups with this much LDS that an XCD of this process holds at a time.
 inline int slots_per_xcd(int lds_bytes) {

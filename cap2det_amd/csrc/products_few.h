@@ -239,17 +239,5 @@ int launch_few(FewArgs p, hipStream_t stream) {
   return c2d_launch_status();
 }
 
-// Up to 16 rows a group.  Few column tiles: 16 columns a workgroup and its eight waves on one chain of segments each, to
-// fill the chip and shorten the chains; many: 32 columns and two waves, whose starts and joins then weigh
-// less (us, 8 waves of 16 columns / 2 waves of 32):  1 x 8192 x 4096 in 8 bits 8.1 / 9.4, 16 x 4096 x 4096 7.7 /
-// 10.2;  64 rows in 64 groups, 2048 x 1024: in 8 bits 40.6 / 18.3, bf16 43.7 / 32.6.
-template <int KIND, bool E5M2, bool VEC, bool OUT16>
-int launch_sixteen_rows(const FewArgs& p, hipStream_t stream) {
-  const double groups = p.offsets ? (p.groups < p.rows ? p.groups : p.rows) : 1;
-  const double tiles = (p.rows / 16.0 + 0.6 * groups) * ((p.n + 15) / 16);
-  if (KIND != F32 && tiles > 700) return launch_few<KIND, E5M2, 1, 2, 2, VEC, OUT16>(p, stream);
-  return launch_few<KIND, E5M2, 1, 1, 8, VEC, OUT16>(p, stream);
-}
-
 }  // namespace
 }  // namespace c2d_pr
