@@ -524,7 +524,7 @@ int launch_tiles(FewArgs a, hipStream_t stream) {
 template <bool E5M2, bool VEC, bool OUT16>
 int launch_fp8(const FewArgs& a, hipStream_t stream) {
   constexpr int KIND = OUT16 ? FP8 : FP8_WIDE;
-  switch (fp8_shape(a.rows, a.n, a.k, a.groups, a.offsets != nullptr, OUT16, VEC)) {
+  switch (fp8_shape(a.rows, a.n, a.k, a.groups, a.offsets != nullptr, OUT16, VEC, c2d_available_cus())) {
     case T16: return launch_few<KIND, E5M2, 1, 1, 8, VEC, OUT16>(a, stream);
     case T16W: return launch_few<KIND, E5M2, 1, 2, 2, VEC, OUT16>(a, stream);
     case T32: return launch_few<KIND, E5M2, 2, 2, 8, VEC, OUT16>(a, stream);

@@ -262,7 +262,7 @@ int launch_tiles(FewArgs a, hipStream_t stream) {
 
 template <int ES, bool TRB, bool VEC, bool OUT16>
 int launch_rows(const FewArgs& a, hipStream_t stream) {
-  const Shape shape = rows_shape(a.rows, a.n, a.k, a.groups, ES, !TRB, VEC);
+  const Shape shape = rows_shape(a.rows, a.n, a.k, a.groups, ES, !TRB, VEC, c2d_available_cus());
   if constexpr (ES == 2 && VEC) {
     if (shape == T256) return launch_tiles<ES, TRB, 2, 4, 4, 2, 1, 2, true, OUT16>(a, stream);
     if (shape == T128W) return launch_tiles<ES, TRB, 2, 4, 2, 2, 1, 2, true, OUT16>(a, stream);

@@ -2,7 +2,7 @@
 //
 // The kernel is the one whose estimated time is least, t = rounds of resident workgroups * (us per stage * stages + us per
 // round), a stage 128 bytes of the contraction (8 bits: a block of k), with the rates that each was measured at.  A round is
-// what 256 CUs hold at a time.
+// what `cus` CUs hold at a time (c2d_available_cus; the rates are those of all 256).
 #pragma once
 
 namespace c2d_pr {
@@ -25,9 +25,9 @@ inline double rounds_of(double tiles, double slots, bool halves) {
 // fill the chip and shorten the chains; many: 32 columns and two waves, whose starts and joins then weigh
 // less (us, 8 waves of 16 columns / 2 waves of 32):  1 x 8192 x 4096 in 8 bits 8.1 / 9.4, 16 x 4096 x 4096 7.7 /
 // 10.2;  64 rows in 64 groups, 2048 x 1024: in 8 bits 40.6 / 18.3, bf16 43.7 / 32.6.
-inline Shape sixteen_rows_shape(int rows, int n, int groups, bool fp32) {
+inline Shape sixteen_rows_shape(int rows, int n, int groups, bool fp32, int cus) {
   const double tiles = (rows / 16.0 + 0.6 * groups) * ((n + 15) / 16);
-  return !fp32 && tiles > 700 ? T16W : T16;
+  return !fp32 && tiles > 700.0 / 256 * cus ? T16W : T16;
 }
 
 // ---- grouped rows, bf16 and fp32
@@ -50,9 +50,9 @@ inline Shape sixteen_rows_shape(int rows, int n, int groups, bool fp32) {
 // 64 x 64 tile 0.56, of 128 x 128 1.9 or, two per CU, 3.8) and has no 256 x 256 tiles, which gain 2.5 % on
 // 4096^3 and lose wherever tiles are few (4 groups of 1024 x 416 x 1024: 241 against 42 in 64 x 64 tiles).
 // (n, k: the result's columns and the contraction)
-inline Shape rows_shape(int rows, int n, int k, int groups_, int es, bool forward, bool vec) {
+inline Shape rows_shape(int rows, int n, int k, int groups_, int es, bool forward, bool vec, int cus) {
   const int groups = groups_ < rows ? groups_ : rows;
-  if (forward && (long long)rows <= 16ll * groups) return sixteen_rows_shape(rows, n, groups, es == 4);
+  if (forward && (long long)rows <= 16ll * groups) return sixteen_rows_shape(rows, n, groups, es == 4, cus);
   // One group's row tiles are known.  Of several a last tile counts for what it costs, on average, and to a round of 128
   // rows a twentieth is added, since a few tiles too many cost another one (8 groups of 625 x 1000 x 1536, input
   // gradient, 258 tiles of 128 x 256: 33.5 us, in 256 x 256 tiles 29.3; of those more are made as halves).
@@ -65,13 +65,13 @@ inline Shape rows_shape(int rows, int n, int k, int groups_, int es, bool forwar
   const double t256 = tiles(256, 256), t128w = tiles(128, 256), t128 = tiles(128, 128);
   // From `lo` at half of `full` to `hi` at all of it, and behind.
   auto between = [](double t, double full, double lo, double hi) { return t >= full ? hi : t <= full / 2 ? lo : lo + (hi - lo) * (2 * t / full - 1); };
-  const double us256 = rounds_of(t256, 256, true) * (between(t256, 256, forward ? 1.12 : 1.3, 1.65) * stages + 6.0);
-  const double us128w = spare * t128w <= 256 ? (forward ? between(t128w, 256, 0.7, 1.03) : between(t128w, 256, 0.85, 1.1)) * stages + 3.5 : 1e30;
+  const double us256 = rounds_of(t256, cus, true) * (between(t256, cus, forward ? 1.12 : 1.3, 1.65) * stages + 6.0);
+  const double us128w = spare * t128w <= cus ? (forward ? between(t128w, cus, 0.7, 1.03) : between(t128w, cus, 0.85, 1.1)) * stages + 3.5 : 1e30;
   const double one = es == 4 ? 1.9 : forward ? 0.57 : 0.66;
-  const double more = es == 4 ? between(t128, 512, 1.9, 3.8) : forward ? between(t128, 512, 0.82, 1.04) : between(t128, 512, 0.87, 1.15);
-  const double us128 = rounds_of(spare * t128, 512, true) * ((t128 <= 256 ? one : more) * stages + 3.5);
-  const double us64 = rounds_of(tiles(64, 64), 256, false) * ((es == 4 ? 0.56 : 0.25) * stages + 3.0);
-  const double us32 = forward ? tiles(32, 32) / 256 * (es == 4 ? 0.4 : 0.29) * stages + 2.5 : 1e30;
+  const double more = es == 4 ? between(t128, 2 * cus, 1.9, 3.8) : forward ? between(t128, 2 * cus, 0.82, 1.04) : between(t128, 2 * cus, 0.87, 1.15);
+  const double us128 = rounds_of(spare * t128, 2 * cus, true) * ((t128 <= cus ? one : more) * stages + 3.5);
+  const double us64 = rounds_of(tiles(64, 64), cus, false) * ((es == 4 ? 0.56 : 0.25) * stages + 3.0);
+  const double us32 = forward ? tiles(32, 32) / cus * (es == 4 ? 0.4 : 0.29) * stages + 2.5 : 1e30;
   const double rest = us64 <= us32 ? us64 : us32, most = us128 <= rest ? us128 : rest;
   if (es == 2 && vec && us256 <= us128w && us256 <= most) return T256;
   if (es == 2 && vec && us128w <= most) return T128W;
@@ -92,19 +92,19 @@ inline Shape rows_shape(int rows, int n, int k, int groups_, int es, bool forwar
 // 64 x 64 tiles 12.4; 16 x 4096 x 4096: 7.7 against 12.5).  An fp32 result doubles the matrix instructions and the
 // registers of a block's products; it has no 256 x 256 tiles, whose registers it would spill, nor have
 // operands that pass through registers on their way to LDS.
-inline Shape fp8_shape(int rows, int n, int k, int groups_, bool ragged, bool out16, bool vec) {
+inline Shape fp8_shape(int rows, int n, int k, int groups_, bool ragged, bool out16, bool vec, int cus) {
   const int groups = !ragged ? 1 : groups_ < rows ? groups_ : rows;
-  if ((long long)rows <= 16ll * groups) return sixteen_rows_shape(rows, n, groups, false);
+  if ((long long)rows <= 16ll * groups) return sixteen_rows_shape(rows, n, groups, false, cus);
   auto tiles = [&](int side) {  // (a group's last row tile counts for what it costs, on average)
     const double down = ragged ? (double)rows / side + 0.4 * groups : (double)((rows + side - 1) / side);
     return down * ((n + side - 1) / side);
   };
   const double kb = (double)(((long long)k + 127) / 128), wide = out16 ? 1.0 : 1.5;
   const double t256 = tiles(256), t128 = tiles(128);
-  const double us256 = rounds_of(t256, 256, true) * ((t256 <= 256 ? 1.5 : 1.95) * kb + 3.5);
-  const double us128 = rounds_of(t128, 512, true) * ((t128 <= 256 ? 0.75 : 1.3) * wide * kb + 3.5);
-  const double us64 = rounds_of(tiles(64), 256, false) * (0.28 * wide * kb + 3.5);
-  const double us32 = tiles(32) / 256 * 0.29 * kb + 2.5;
+  const double us256 = rounds_of(t256, cus, true) * ((t256 <= cus ? 1.5 : 1.95) * kb + 3.5);
+  const double us128 = rounds_of(t128, 2 * cus, true) * ((t128 <= cus ? 0.75 : 1.3) * wide * kb + 3.5);
+  const double us64 = rounds_of(tiles(64), cus, false) * (0.28 * wide * kb + 3.5);
+  const double us32 = tiles(32) / cus * 0.29 * kb + 2.5;
   if (out16 && vec && us256 <= us128 && us256 <= us64 && us256 <= us32) return T256;
   if (us128 <= us64 && us128 <= us32) return T128;
   return us64 <= us32 ? T64 : T32;
@@ -113,7 +113,8 @@ inline Shape fp8_shape(int rows, int n, int k, int groups_, bool ragged, bool ou
 // ---- weight gradient
 //
 // The rows of a group are the contraction, dealt to `splits` workgroups where the tiles of dw are few; a round ends with
-// the tile's way to memory, and splits with the sum over them.
+// the tile's way to memory, and splits with the sum over them.  The rounds are those of the whole chip: a plan that followed
+// c2d_set_available_cus would change the workspace under a program that keeps one.
 struct WgradPlan { int side, splits; };
 inline WgradPlan wgrad_plan(int groups, int rows, int n, int k, int es) {
   const double stages = ((double)rows / groups * es + 127) / 128, mb = 4e-6 * groups * n * k;
