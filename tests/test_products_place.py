@@ -122,7 +122,7 @@ def test_the_last_round_of_one_long_group_is_made_as_halves(host, rows, n, ragge
 def test_ragged_groups(host, bm, halves, bn, slots):
   r = random.Random(bm + bn + slots)
   cut = 0
-  for _ in range(15):
+  for _ in range(40):
     groups = r.choice((1, 2, 5, 32, 70, 150))
     rows = r.randrange(1, 9000)
     cuts = sorted(r.randrange(0, rows + 1) for _ in range(groups + 1))
