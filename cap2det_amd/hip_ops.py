@@ -1060,7 +1060,10 @@ def fp8_matmul(a, a_scale, b, b_scale, out=None, out_dtype=torch.bfloat16, bias=
 
 def grouped_matmul_fp8(a, a_scale, b, b_scale, offsets, out=None, out_dtype=torch.bfloat16, bias=None, relu=False):
   """fp8_matmul with one weight matrix per group of rows: b [groups, n, k], b_scale [groups, ceil(n / 128),
-  ceil(k / 128)], bias [groups, n]."""
+  ceil(k / 128)], bias [groups, n].  The input gradient is the same product on b.transpose(1, 2).contiguous() and
+  b_scale.transpose(1, 2).contiguous(), which a program makes once per update of the weights; the weight gradient is
+  grouped_matmul_wgrad on the values before their quantisation (it sums over rows, and blocks of 128 rows would not
+  end where groups do)."""
   device = _device()
   if not (bias is None and _tensors(a, a_scale, b, b_scale, offsets) and a.dim() == 2 and b.dim() == 3 and b.shape[0] > 0 and
           a.get_device() == b.get_device() == a_scale.get_device() == b_scale.get_device() == offsets.get_device() == device and

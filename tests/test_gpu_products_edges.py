@@ -171,3 +171,19 @@ def test_as_many_groups_as_are_taken():
   assert torch.equal(ops.grouped_matmul_wgrad(x, dy, offs), want)
   y = ops.grouped_matmul_fp8(x.to(E4M3), torch.ones(t, 1, device="cuda"), w.to(E4M3), torch.ones(groups, 1, 1, device="cuda"), offs)
   assert torch.equal(y, (w[of].float() * x[:, None].float()).sum(-1).to(BF16))
+
+
+def test_the_input_gradient_of_experts_in_8_bits_with_transposed_weights():
+  """dx_e = dy_e . w_e through the grouped product on each w_e^T: square blocks transpose with their matrix."""
+  gen = _gen(54)
+  offsets = up.offsets_of([70, 0, 300, 1])
+  t, n, k = offsets[-1], 264, 392
+  dy = torch.randn(t, n, generator=gen, device="cuda").to(BF16)
+  w = torch.randn(4, n, k, generator=gen, device="cuda") * n ** -0.5
+  q, s = ops.fp8_quantize(w, 128)
+  g, g_s = ops.fp8_quantize(dy, 1, E5M2)
+  qt, st = q.transpose(1, 2).contiguous(), s.transpose(1, 2).contiguous()
+  assert torch.equal(qt.view(torch.uint8), ops.fp8_quantize(w.transpose(1, 2).contiguous(), 128)[0].view(torch.uint8))
+  dx = ops.grouped_matmul_fp8(g, g_s, qt, st, _offs(offsets), out_dtype=F32)
+  dg, dw = up.dequantized(g, g_s, 1), up.dequantized(q, s, 128).transpose(1, 2)
+  up.assert_within(dx, up.grouped(dg, dw, offsets), up.sum_bound(128 + 3 + 2, up.grouped(dg.abs(), dw.abs(), offsets)))
