@@ -148,7 +148,8 @@ struct QuantArgs {
 
 // Blocks of 1 x 128: 16 lanes a block, 8 elements a lane, `span` blocks a workgroup (64; 32 or 16 where that many would
 // leave CUs without work), all of whose loads are issued before the first is used.  What bounds it is memory: 32768 x
-// 8192 bf16 in 145 us, 5.6 TB/s, where a copy reaches 5.1.
+// 8192 bf16 in 147 us in a replayed graph and 150-174 launched one by one (5.5 and 4.6-5.4 TB/s of twice as much read as
+// written, where a copy reaches 5.15).
 template <class T, bool E5M2>
 __global__ __launch_bounds__(256) void quantize_rows_kernel(QuantArgs a) {
   const int lane16 = threadIdx.x & 15, slot = threadIdx.x >> 4;
@@ -337,9 +338,10 @@ __device__ __forceinline__ f32x16 fp8_half(const i32x4 (&b)[4], const i32x4 (&a)
 // The stages of A go round D buffers, those of B round D + 1: while a stage is multiplied, the next of A and
 // the next two of B are on their way (D = 2; five buffers are what the LDS holds of 256 x 256 tiles).  Within a
 // stage the loads are issued between the matrix instructions of its first tiles, and a tile's scaling runs under
-// the matrix instructions of the next: 8192^3 in 503 us, 2190 TFLOP/s, where the library's product with one scale
-// for the whole matrix reaches 2680; with the loads in front and the scaling behind its own products 652.  The
-// matrix pipe is busy 57 % of that time, LDS 23 %: the wait at the stages' barriers is what is left.
+// the matrix instructions of the next: 8192^3 in 508-515 us in a replayed graph, 530-537 launched one by one (2150 and 2060
+// TFLOP/s; in the first 10 ms of such a load up to 655), where the library's product with one scale for the whole matrix reaches
+// 2680-2790; with the loads in front and the scaling behind its own products 652.  The
+// matrix pipe is busy 55 % of that time, LDS 22 %: the wait at the stages' barriers is what is left.
 //
 // KG > 1: KG groups of WM x WN waves share the tile, group g taking the stages g, g + KG, ..; their sums are
 // joined through LDS, in the groups' order.  A stage of a small tile is a chain of waits (barrier, LDS read, two

@@ -18,7 +18,8 @@ struct WgradArgs {
 // The stages of A go round D buffers, those of B round D + 1: while a stage is multiplied, the next of A and
 // the next two of B are on their way (D = 2; five buffers are what the LDS holds of 256 x 256 tiles, and a load takes
 // longer than a stage).  B are the weights, which come from memory, each group's own, where rows come from L2
-// for all but one of their column tiles (8192^3: 851 us, with the third buffer A's 874; its input gradient 870, 906).
+// for all but one of their column tiles (8192^3: 851 us, with the third buffer A's 874; its input gradient 870, 906;
+// on other cards of the kind 851-881 and 870-925).
 // One barrier per stage; the loads are issued between the matrix instructions of its first half, since a burst
 // of them behind the barrier holds up every wave of the workgroup.
 // KG > 1: KG groups of WM x WN waves share the tile, group g taking the stages g, g + KG, ..
@@ -187,7 +188,7 @@ __global__ __launch_bounds__(WM * WN * KG * 64, 2) void grouped_wgrad_kernel(Wgr
   __shared__ __attribute__((aligned(1024))) char smem[KG * C::RING];
   // Workgroups go round the 8 XCDs: of every 256 tiles XCD x takes the x-th eighth, so that a group's rows come through
   // the L2 of an XCD or two instead of all eight, and every XCD meets long groups and short ones (32 groups of
-  // about 512 x 2048 x 2048: 242 us; tiles in their order 252, 576 MB fetched of 134; an eighth of all tiles 271.  One
+  // about 512 x 2048 x 2048: 242 us, on other cards to 262; tiles in their order 252, 576 MB fetched of 134; an eighth of all tiles 271.  One
   // group of 16384 x 2048 x 2048: 138 us, in their order 165).
   const int tiles = a.ntiles * a.ktiles, total = tiles * a.splits * a.groups;
   const unsigned wg = workgroup();

@@ -186,7 +186,8 @@ __device__ __forceinline__ void clear_rest(const Place& p, T* y, long long ldy, 
 //
 // UNSEEN: the load to LDS is written as an instruction that the compiler does not look into.  It waits for
 // every such load that it knows of before each transposed LDS read, which is the whole latency of the next stage
-// at every step of 16 k (input gradient 8192^3 in 256 x 256 tiles: 1054 us, unseen 921; in 128 x 128 tiles 1341, 1113);
+// at every step of 16 k (input gradient 8192^3 in 256 x 256 tiles: 1054 us, unseen 921, with the loads between the matrix
+// instructions as they are now 870-925; in 128 x 128 tiles 1341, 1113);
 // stage_barrier waits for what is needed.
 template <int ES, bool TR, int R, int NTH, bool VEC, bool UNSEEN = false>
 struct Tile {

@@ -201,7 +201,7 @@ __global__ __launch_bounds__(KW * 64) void few_rows_kernel(FewArgs p) {
 #pragma unroll
     for (int j = 0; j < NT; ++j) *(f32x4*)&part[wave][16 * i + l16][16 * j + 4 * q] = acc[i][j];
   __syncthreads();
-  // the sums in the waves' order; eight lanes a row, four columns each
+  // the sums in the waves' order; BN / 4 lanes a row, four columns each
   for (int t = threadIdx.x; t < BM * (BN / 4); t += KW * 64) {
     const int m = t / (BN / 4), col = (t % (BN / 4)) * 4;
     if (m >= a_rows) break;
