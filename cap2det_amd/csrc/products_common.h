@@ -137,7 +137,7 @@ __device__ __forceinline__ Place place_tile(const int* __restrict__ offsets, int
   }
   int before = 0;
   if (groups > 64) carry = 0;
-  for (int base = 0;; base += 64) {
+  for (int base = 0; base < groups; base += 64) {
     if (groups > 64) {
       s = lane_span(offsets, groups, rows, base, &carry);
       upto_full = lane_prefix_sum(full_tiles_of<BM, HALVES>(s.hi - s.lo));
@@ -156,6 +156,8 @@ __device__ __forceinline__ Place place_tile(const int* __restrict__ offsets, int
     }
     before += __builtin_amdgcn_readlane(upto, 63);
   }
+  p.live = false;  // (offsets that somebody changed since they were counted: no tile, rather than a search without end)
+  return p;
 }
 
 // Rows in no group := 0, by the workgroups that have no tile.
