@@ -338,7 +338,7 @@ __device__ __forceinline__ f32x16 fp8_half(const i32x4 (&b)[4], const i32x4 (&a)
 // The stages of A go round D buffers, those of B round D + 1: while a stage is multiplied, the next of A and
 // the next two of B are on their way (D = 2; five buffers are what the LDS holds of 256 x 256 tiles).  Within a
 // stage the loads are issued between the matrix instructions of its first tiles, and a tile's scaling runs under
-// the matrix instructions of the next: 8192^3 in 508-515 us in a replayed graph, 530-537 launched one by one (2150 and 2060
+// the matrix instructions of the next: 8192^3 in 493-515 us in a replayed graph, 517-537 launched one by one (2180 and 2090
 // TFLOP/s; in the first 10 ms of such a load up to 655), where the library's product with one scale for the whole matrix reaches
 // 2680-2790; with the loads in front and the scaling behind its own products 652.  The
 // matrix pipe is busy 55 % of that time, LDS 22 %: the wait at the stages' barriers is what is left.
